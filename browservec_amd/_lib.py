@@ -78,6 +78,27 @@ class IndexStats(ctypes.Structure):
     ]
 
 
+def _args(name: str, fields: str) -> type:
+    """A ctypes struct from "type name" words in the header's order."""
+    types = {"u32": ctypes.c_uint32, "u64": ctypes.c_uint64, "f32": ctypes.c_float, "f64": ctypes.c_double,
+             "ptr": ctypes.c_void_p}
+    words = fields.split()
+    return type(name, (ctypes.Structure,), {"_fields_": [(n, types[t]) for t, n in zip(words[::2], words[1::2])]})
+
+
+LinearArgs = _args("LinearArgs", """u32 size u32 dtype u32 out_dtype u32 activation u64 m u32 n u32 k ptr x ptr w ptr bias
+    ptr residual ptr y u64 x_stride u64 w_stride u64 residual_stride u64 y_stride""")
+RotaryArgs = _args("RotaryArgs", """u32 size u32 dtype u32 heads_q u32 heads_k u32 head_dim u32 rot_dim u32 interleaved
+    u32 table_rows u64 tokens ptr table ptr positions ptr q ptr k ptr q_out ptr k_out u64 q_stride u64 q_head_stride
+    u64 k_stride u64 k_head_stride u64 q_out_stride u64 q_out_head_stride u64 k_out_stride u64 k_out_head_stride""")
+RotaryScaling = _args("RotaryScaling", """u32 size u32 kind f64 base f64 factor f64 original_rows f64 low_turns
+    f64 high_turns f64 magnitude""")
+AttentionArgs = _args("AttentionArgs", """u32 size u32 dtype u32 heads_q u32 heads_k u32 head_dim u32 causal u32 batch
+    u32 max_q u32 max_k f32 scale u64 tokens_q u64 tokens_k ptr q ptr k ptr v ptr o ptr cu_q ptr cu_k u64 q_stride
+    u64 q_head_stride u64 k_stride u64 k_head_stride u64 v_stride u64 v_head_stride u64 o_stride u64 o_head_stride""")
+NormArgs = _args("NormArgs", """u32 size u32 dtype u32 out_dtype u32 weight_dtype u32 norm u32 pool u32 unit u32 batch
+    u32 dim f32 eps u64 tokens ptr x ptr weight ptr bias ptr cu ptr y u64 x_stride u64 y_stride""")
+
 vp = ctypes.c_void_p
 u32 = ctypes.c_uint32
 u64 = ctypes.c_uint64
@@ -126,6 +147,16 @@ SIGNATURES = {
     "bv_index_export_probe_scores": [vp, vp, u32, vp],
     "bv_index_save_section": [vp, vp, u64, vp],
     "bv_index_load_section": [vp, vp, u64, u64, vp, u64],
+    "bv_embed_create": [vp, ctypes.POINTER(vp)],
+    "bv_embed_destroy": [vp],
+    "bv_embed_set_stream": [vp, vp],
+    "bv_embed_stream": [vp, ctypes.POINTER(vp)],
+    "bv_embed_sync": [vp],
+    "bv_embed_linear": [vp, vp],
+    "bv_embed_rotary": [vp, vp],
+    "bv_embed_rotary_table": [vp, u32, u32, vp, u64],
+    "bv_embed_attention": [vp, vp],
+    "bv_embed_norm": [vp, vp],
 }
 _RESTYPE = {"bv_last_error": ctypes.c_char_p}
 

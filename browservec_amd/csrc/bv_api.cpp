@@ -19,6 +19,7 @@
 #include <string>
 #include <vector>
 
+#include "bv_host.h"
 #include "bv_kernels.h"
 
 using namespace bvk;
@@ -26,7 +27,7 @@ using namespace bvk;
 // ------------------------------------------------------------------ errors
 static thread_local std::string g_err;
 
-static int fail(int code, const char *fmt, ...) {
+int bvk::fail(int code, const char *fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -36,15 +37,13 @@ static int fail(int code, const char *fmt, ...) {
     return code;
 }
 
-struct bv_device {
-    int ordinal = 0;
-    hipDeviceProp_t prop{};
-    bool lost = false;
-    bool inject_append_oom = false;  // bv_debug_inject: fail the next append's allocation
-    bool inject_append_late = false; // bv_debug_inject: fail the next append after its rows are encoded
-    bool inject_slots_oom = false;   // bv_debug_inject: fail the next slot scan's allocation
-    void *scratch = nullptr;         // this GPU's copy of the no-allocation scratch array
-};
+int bvk::hip_fail(bv_device *dev, hipError_t e, const char *what) {
+    if (e == hipErrorOutOfMemory) return fail(BV_E_OOM, "%s: out of device memory", what);
+    if (dev && (e == hipErrorIllegalAddress || e == hipErrorLaunchFailure || e == hipErrorECCNotCorrectable ||
+                e == hipErrorNoDevice))
+        dev->lost = true;
+    return fail(BV_E_HIP, "%s: %s", what, hipGetErrorString(e));
+}
 
 // ------------------------------------------------- no-allocation scratch --
 // The fused scan's scratch for bv_index_search_device_noalloc lives in a
@@ -66,54 +65,6 @@ static void *resolve_scratch(int ordinal) {
     }
     return g_scratch_ptr[ordinal];
 }
-
-static int hip_fail(bv_device *dev, hipError_t e, const char *what) {
-    if (e == hipErrorOutOfMemory) return fail(BV_E_OOM, "%s: out of device memory", what);
-    if (dev && (e == hipErrorIllegalAddress || e == hipErrorLaunchFailure || e == hipErrorECCNotCorrectable ||
-                e == hipErrorNoDevice))
-        dev->lost = true;
-    return fail(BV_E_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
-#define HIPX(dev, expr, what)                        \
-    do {                                             \
-        hipError_t _e = (expr);                      \
-        if (_e != hipSuccess) return hip_fail((dev), _e, (what)); \
-    } while (0)
-
-// -------------------------------------------------------- device buffers
-struct DevBuf {
-    void *p = nullptr;
-    size_t cap = 0;
-    ~DevBuf() { release(); }
-    void release() {
-        if (p) (void)hipFree(p);
-        p = nullptr;
-        cap = 0;
-    }
-    // Grow to at least `bytes`, preserving the first `keep` bytes.
-    hipError_t ensure(size_t bytes, size_t keep, hipStream_t s, bool geometric = true) {
-        if (bytes <= cap) return hipSuccess;
-        size_t ncap = geometric ? std::max(bytes, cap + cap / 2) : bytes;
-        ncap = (ncap + 255) & ~size_t(255);
-        void *np = nullptr;
-        hipError_t e = hipMalloc(&np, ncap);
-        if (e != hipSuccess) return e;
-        if (p && keep) {
-            e = hipMemcpyAsync(np, p, keep, hipMemcpyDeviceToDevice, s);
-            if (e == hipSuccess) e = hipStreamSynchronize(s);
-            if (e != hipSuccess) {
-                (void)hipFree(np);
-                return e;
-            }
-        }
-        if (p) (void)hipFree(p);
-        p = np;
-        cap = ncap;
-        return hipSuccess;
-    }
-    template <class T> T *as() const { return (T *)p; }
-};
 
 struct HostBuf {
     void *p = nullptr;

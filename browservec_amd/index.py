@@ -45,6 +45,7 @@ class DeviceContext:
 
     def __init__(self, ordinal: int = 0):
         self.lib = L.load()
+        self.ordinal = ordinal
         h = ctypes.c_void_p()
         L.check(self.lib.bv_device_open(ordinal, ctypes.byref(h)))
         self.handle = h

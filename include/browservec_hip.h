@@ -331,6 +331,216 @@ int bv_graph_search(bv_graph *g, const float *queries, uint32_t nq, uint32_t k, 
 int bv_graph_search_beams(bv_graph *g, const float *queries, uint32_t nq, const uint32_t *entries,
                           uint32_t n_entries, uint32_t ef, uint32_t iter_cap, float *beam_dist, uint32_t *beam_id);
 
+/* ---- an embedding model's operators ------------------------------------------ */
+/* What turns text into the vectors an index holds, beside it on the GPU: the
+ * reference's embedder runs in another library (src/embed/transformers.ts),
+ * these are the operators such a model's forward pass is made of.  Every
+ * pointer is device memory unless it says otherwise; a call checks its
+ * arguments, enqueues kernels on the handle's stream and returns without
+ * waiting.  Matrices and heads have contiguous last dimensions and strides in
+ * elements (0: packed); every alignment and size works, 16-byte aligned rows
+ * run fastest.  Sums, softmax statistics and norms are 32-bit floats; results
+ * are rounded once to the output's type, and the same call on the same inputs
+ * gives the same bits.  Outputs may not overlap inputs except where a
+ * description allows it.
+ *
+ * A handle is used by one thread at a time.  Its workspaces, one for each
+ * stream it is used on, grow with the largest call so far and are held until
+ * the handle is destroyed: after one call of a size on a stream, further calls
+ * of it there allocate nothing and launch only kernels, so they can be
+ * captured into a HIP graph. */
+#define BV_F32 0
+#define BV_F16 1
+#define BV_BF16 2
+
+typedef struct bv_embed bv_embed;
+
+/* A handle with a stream of its own (not ordered with the null stream). */
+int bv_embed_create(bv_device *dev, bv_embed **out);
+/* Waits for the device. */
+int bv_embed_destroy(bv_embed *e);
+/* Run further calls on another stream (hipStream_t; NULL is the device's
+ * default stream), an index's (bv_index_stream) to append or search without
+ * waiting in between.  Orders nothing: calls on two streams may run at once. */
+int bv_embed_set_stream(bv_embed *e, void *stream);
+int bv_embed_stream(bv_embed *e, void **stream);
+int bv_embed_sync(bv_embed *e);
+
+/* y = act(x w^T + bias) + residual: x [m][k], w [n][k] and bias [n] in dtype
+ * (BV_F16 or BV_BF16), residual and y [m][n] in out_dtype (dtype or BV_F32).
+ * bias and residual may be NULL; residual may be y itself. */
+#define BV_ACT_NONE 0
+#define BV_ACT_RELU 1
+#define BV_ACT_GELU 2      /* x Phi(x)                                               */
+#define BV_ACT_GELU_TANH 3 /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2        */
+#define BV_ACT_SILU 4      /* x / (1 + exp(-x))                                      */
+typedef struct bv_embed_linear_args {
+    uint32_t size;        /* sizeof(bv_embed_linear_args) */
+    uint32_t dtype;
+    uint32_t out_dtype;
+    uint32_t activation;  /* BV_ACT_* */
+    uint64_t m;
+    uint32_t n;
+    uint32_t k;
+    const void *x;
+    const void *w;
+    const void *bias;
+    const void *residual;
+    void *y;
+    uint64_t x_stride;    /* elements from a row to the next; 0: packed */
+    uint64_t w_stride;
+    uint64_t residual_stride;
+    uint64_t y_stride;
+} bv_embed_linear_args;
+int bv_embed_linear(bv_embed *e, const bv_embed_linear_args *args);
+
+/* Rotary positions: the first rot_dim elements of every head turn in pairs,
+ * (a, b) -> (a cos - b sin, b cos + a sin); the others are copied.  Pairs are
+ * elements i and i + rot_dim/2, or 2i and 2i+1 with interleaved.  table holds
+ * a row per position, [table_rows][rot_dim/2] pairs (cos, sin) of 32-bit floats
+ * (bv_embed_rotary_table); positions one int32 per token (NULL: 0, 1, ...).  A
+ * position outside the table turns its token's elements into NaN.  q
+ * [tokens][heads_q][head_dim] and k [tokens][heads_k][head_dim] in dtype; k may
+ * be NULL with heads_k 0.  q_out may be q and k_out k, with the same strides. */
+typedef struct bv_embed_rotary_args {
+    uint32_t size;        /* sizeof(bv_embed_rotary_args) */
+    uint32_t dtype;
+    uint32_t heads_q;
+    uint32_t heads_k;
+    uint32_t head_dim;
+    uint32_t rot_dim;     /* even, at most head_dim */
+    uint32_t interleaved;
+    uint32_t table_rows;
+    uint64_t tokens;
+    const float *table;
+    const int32_t *positions;
+    const void *q;
+    const void *k;
+    void *q_out;
+    void *k_out;
+    uint64_t q_stride;    /* elements from a token to the next; 0: packed */
+    uint64_t q_head_stride;
+    uint64_t k_stride;
+    uint64_t k_head_stride;
+    uint64_t q_out_stride;
+    uint64_t q_out_head_stride;
+    uint64_t k_out_stride;
+    uint64_t k_out_head_stride;
+} bv_embed_rotary_args;
+int bv_embed_rotary(bv_embed *e, const bv_embed_rotary_args *args);
+
+/* The table of bv_embed_rotary in host memory: cos and sin of position times
+ * frequency in 64 bits, rounded to 32.  Pair i's frequency is
+ * f = base^(-2i/rot_dim), scaled for contexts `factor` times the original:
+ *   BV_ROTARY_NONE    f
+ *   BV_ROTARY_LINEAR  f / factor
+ *   BV_ROTARY_BASE    f of the base times factor^(rot_dim/(rot_dim-2))
+ *   BV_ROTARY_PARTS   f (g + (1-g)/factor): g = 1 for pairs that turn at least
+ *                     high_turns times over original_rows positions, 0 for
+ *                     those that turn at most low_turns times, linear between
+ * magnitude multiplies cos and sin (0: 1).  n_floats must be
+ * table_rows * rot_dim. */
+#define BV_ROTARY_NONE 0
+#define BV_ROTARY_LINEAR 1
+#define BV_ROTARY_BASE 2
+#define BV_ROTARY_PARTS 3
+typedef struct bv_embed_rotary_scaling {
+    uint32_t size;        /* sizeof(bv_embed_rotary_scaling) */
+    uint32_t kind;        /* BV_ROTARY_* */
+    double base;
+    double factor;
+    double original_rows;
+    double low_turns;
+    double high_turns;
+    double magnitude;
+} bv_embed_rotary_scaling;
+int bv_embed_rotary_table(const bv_embed_rotary_scaling *scaling, uint32_t table_rows, uint32_t rot_dim, float *table,
+                          uint64_t n_floats);
+
+/* o = softmax(scale q k^T) v per packed sequence and head: sequence s has the
+ * queries cu_q[s] to cu_q[s+1] of q [tokens_q][heads_q][head_dim] and the keys
+ * cu_k[s] to cu_k[s+1] of k, v [tokens_k][heads_k][head_dim] (dtype BV_F16 or
+ * BV_BF16; head_dim at most 256; heads_q a multiple of heads_k, query head h
+ * reads key head h / (heads_q/heads_k)).  cu_q, cu_k: batch + 1 ascending
+ * int32, clipped to the tokens there are.  causal: a sequence's last query
+ * sees its last key, each query before it one key less.  A query that sees no
+ * key gives zeros.  Keys and values that a query does not see have no effect
+ * on it, whatever they hold.  scale 0: 1/sqrt(head_dim).  max_q and max_k are
+ * the longest lengths as far as the caller knows them (0: unknown); they only
+ * steer how the work is split, never which of it is done.  Queries outside
+ * every sequence leave their rows of o as they are. */
+typedef struct bv_embed_attention_args {
+    uint32_t size;        /* sizeof(bv_embed_attention_args) */
+    uint32_t dtype;
+    uint32_t heads_q;
+    uint32_t heads_k;
+    uint32_t head_dim;
+    uint32_t causal;
+    uint32_t batch;
+    uint32_t max_q;
+    uint32_t max_k;
+    float scale;
+    uint64_t tokens_q;
+    uint64_t tokens_k;
+    const void *q;
+    const void *k;
+    const void *v;
+    void *o;
+    const int32_t *cu_q;
+    const int32_t *cu_k;
+    uint64_t q_stride;    /* elements from a token to the next; 0: packed */
+    uint64_t q_head_stride;
+    uint64_t k_stride;
+    uint64_t k_head_stride;
+    uint64_t v_stride;
+    uint64_t v_head_stride;
+    uint64_t o_stride;
+    uint64_t o_head_stride;
+} bv_embed_attention_args;
+int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *args);
+
+/* The norm of token rows and their pooling to one vector a sequence.
+ * x [tokens][dim] in dtype; each row becomes
+ *   BV_NORM_NONE   x
+ *   BV_NORM_LAYER  (x - mean) / sqrt(var + eps)
+ *   BV_NORM_RMS    x / sqrt(mean(x^2) + eps)
+ * times weight plus bias ([dim] in weight_dtype, each may be NULL).  With
+ * BV_POOL_NONE y holds those rows, [tokens][dim] in out_dtype (y may be x where
+ * the types and strides are the same).  Otherwise y [batch][dim], out_dtype
+ * BV_F32, holds per sequence cu[s] to cu[s+1] (batch + 1 ascending int32,
+ * clipped to the tokens there are) their mean, the first or the last of them,
+ * and with unit divided by its 2-norm: the rows bv_index_append_device and the
+ * queries bv_index_search_device take.  An empty sequence gives zeros, a
+ * vector of norm zero stays as it is. */
+#define BV_NORM_NONE 0
+#define BV_NORM_LAYER 1
+#define BV_NORM_RMS 2
+#define BV_POOL_NONE 0
+#define BV_POOL_MEAN 1
+#define BV_POOL_FIRST 2
+#define BV_POOL_LAST 3
+typedef struct bv_embed_norm_args {
+    uint32_t size;        /* sizeof(bv_embed_norm_args) */
+    uint32_t dtype;
+    uint32_t out_dtype;
+    uint32_t weight_dtype;
+    uint32_t norm;        /* BV_NORM_* */
+    uint32_t pool;        /* BV_POOL_* */
+    uint32_t unit;
+    uint32_t batch;
+    uint32_t dim;
+    float eps;
+    uint64_t tokens;
+    const void *x;
+    const void *weight;
+    const void *bias;
+    const int32_t *cu;
+    void *y;
+    uint64_t x_stride;    /* elements from a row to the next; 0: packed */
+    uint64_t y_stride;
+} bv_embed_norm_args;
+int bv_embed_norm(bv_embed *e, const bv_embed_norm_args *args);
+
 #ifdef __cplusplus
 }
 #endif
