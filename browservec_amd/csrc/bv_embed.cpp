@@ -242,7 +242,9 @@ extern "C" int bv_embed_linear(bv_embed *e, const bv_embed_linear_args *args) {
     l.ldw = a.w_stride;
     l.ldr = a.residual_stride;
     l.ldy = a.y_stride;
-    HIPX(e->dev, launch_linear(l, e->stream), "linear kernel");
+    void *ws = nullptr;
+    OK_OR_RETURN(embed_workspace(e, linear_workspace(l), &ws));
+    HIPX(e->dev, launch_linear(l, ws, e->stream), "linear kernel");
     return BV_OK;
 }
 

@@ -19,7 +19,9 @@ struct LinearArgs {
     void *y;
     uint64_t ldx, ldw, ldr, ldy;
 };
-hipError_t launch_linear(const LinearArgs &a, hipStream_t s);
+// Bytes of workspace that a call needs (rows laid out for the matrix cores).
+size_t linear_workspace(const LinearArgs &a);
+hipError_t launch_linear(const LinearArgs &a, void *ws, hipStream_t s);
 
 // ------------------------------------------------------------- attention --
 struct AttentionArgs {

@@ -1,61 +1,424 @@
-// y = act(x w^T + bias) + residual for an embedding model's layers.
+// y = act(x w^T + bias) + residual for an embedding model's layers, on the
+// matrix cores.
+//
+// The products are computed transposed, w's rows as the matrix instructions'
+// first operand and x's as their second: a lane then holds four neighbouring
+// columns of one of y's rows, which leave it as one piece.
 #include "bv_embed.h"
 #include "bv_embed_device.h"
+#include "bv_mfma.h"
 
 #include <algorithm>
 
 namespace bvk {
 namespace {
 
-__device__ __forceinline__ float activate(float y, int act) {
-    switch (act) {
-    case 1: return fmaxf(y, 0.0f) + (y != y ? y : 0.0f);
-    case 2: return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
-    case 3: return 0.5f * y * (1.0f + tanhf(0.79788456080286536f * (y + 0.044715f * y * y * y)));
-    case 4: return y / (1.0f + expf(-y));
-    default: return y;
-    }
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ v16f mfma32(f16x8 a, f16x8 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma32(bf16x8 a, bf16x8 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma16(f16x8 a, f16x8 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma16(bf16x8 a, bf16x8 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 16 x 16 results a workgroup, the operands in tiles of 16 through LDS.
-template <class T, class O>
-__global__ __launch_bounds__(256) void linear_tile(LinearArgs a, uint64_t first) {
-    __shared__ float xs[16][17], ws[16][17];
-    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint64_t m0 = first + (uint64_t)blockIdx.y * 16, n0 = (uint64_t)blockIdx.x * 16;
-    const T *x = (const T *)a.x, *w = (const T *)a.w;
-    float acc = 0;
-    for (uint32_t k0 = 0; k0 < a.k; k0 += 16) {
-        const bool in = k0 + tx < a.k;
-        xs[ty][tx] = in && m0 + ty < a.m ? (float)x[(m0 + ty) * a.ldx + k0 + tx] : 0.0f;
-        ws[ty][tx] = in && n0 + ty < a.n ? (float)w[(n0 + ty) * a.ldw + k0 + tx] : 0.0f;
-        __syncthreads();
+// The activations are y * sigmoid(t), with t / log(2) = y q(y^2):
+//   SILU       q = log2(e)
+//   GELU_TANH  q = log2(e) 2 sqrt(2/pi) (1 + 0.044715 y^2)
+//   GELU       Phi(y) = sigmoid(log(Phi(y) / Phi(-y))), whose argument over y is
+//              smooth in y^2: a polynomial of degree 6 fitted on |y| <= 5.5 so
+//              that the result is within 1.7e-7 max(1, |y|) everywhere (y^2 is
+//              clamped past it, where Phi is 0 or 1 to 2e-8)
+// One exponential and one reciprocal each: with 64 columns of 32 rows a lane,
+// the epilogue's arithmetic is a third of the time of a product with k = 1024
+// (erff took as long as the product).
+__device__ __forceinline__ float times_sigmoid(float y, float q) {
+    return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y * q));
+}
+__device__ __forceinline__ float gelu(float y) {
+    const float u = fminf(y * y, 30.25f);
+    float q = 5.209913833681412e-09f;
+    q = fmaf(q, u, -3.8504521171489614e-07f);
+    q = fmaf(q, u, 1.1452433682279661e-05f);
+    q = fmaf(q, u, -1.5938944125082344e-04f);
+    q = fmaf(q, u, -9.559283353155479e-05f);
+    q = fmaf(q, u, 1.0483857989311218e-01f);
+    q = fmaf(q, u, 2.3022072315216064f);
+    return times_sigmoid(y, q);
+}
+__device__ __forceinline__ void activate8(float (&f)[8], int act) {
+    switch (act) {  // the same for the whole launch
+    case 1:
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc = fmaf(xs[ty][i], ws[tx][i], acc);
-        __syncthreads();
+        for (int i = 0; i < 8; i++) f[i] = f[i] < 0.0f ? 0.0f : f[i];
+        break;
+    case 2:
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = gelu(f[i]);
+        break;
+    case 3:
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = times_sigmoid(f[i], fmaf(f[i] * f[i], 0.10294324f, 2.3022082f));
+        break;
+    case 4:
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = times_sigmoid(f[i], 1.44269504f);
+        break;
+    default: break;
     }
-    const uint64_t m = m0 + ty, n = n0 + tx;
-    if (m >= a.m || n >= a.n) return;
-    if (a.bias) acc += (float)((const T *)a.bias)[n];
-    acc = activate(acc, a.act);
-    if (a.residual) acc += (float)((const O *)a.residual)[m * a.ldr + n];
-    ((O *)a.y)[m * a.ldy + n] = (O)acc;
 }
 
-template <class T, class O>
-hipError_t linear_of(const LinearArgs &a, hipStream_t s) {
-    for (uint64_t m = 0; m < a.m; m += 16 * 32768) {
-        const dim3 grid((a.n + 15) / 16, (uint32_t)std::min<uint64_t>((a.m - m + 15) / 16, 32768));
-        linear_tile<T, O><<<grid, 256, 0, s>>>(a, m);
+// The end of eight neighbouring results of a row, columns n on: residual,
+// rounding, store.
+template <class O>
+__device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_t n, float (&f)[8]) {
+    const int left = (int)min(8u, a.n - n);
+    if (a.residual) {
+        const O *r = (const O *)a.residual + m * a.ldr + n;
+        if (left == 8) {
+            float g[8];
+            load8(r, g);
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] += g[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] += (float)r[min(i, left - 1)];
+        }
+    }
+    store8((O *)a.y + m * a.ldy + n, left, f);
+}
+
+// ------------------------------------------------------------------ tiles --
+// A workgroup of four waves computes BM x BN results, its waves a quarter
+// each (BM/2 x BN/2).  Tiles of BK columns of x and w stream through ST buffers
+// in LDS, loaded straight into it: in every step a wave waits for its share of
+// the oldest tile, meets the others at a barrier (which also says that the
+// buffer of the step before is free), starts the loads of the tile ST - 1
+// steps ahead and multiplies.
+//
+// LDS rows hold BK elements, in 16-byte chunks; chunk c of row r lies at
+// c ^ swizzle(r), so that eight lanes that read the same chunk of consecutive
+// rows cover all banks.  Loads put lane i's chunk at a fixed place, so the
+// swizzle is applied to the address they load from.
+template <int BK>
+__device__ __forceinline__ uint32_t swizzle(uint32_t row) {
+    return BK == 64 ? row & 7 : (row >> 1) & 3;
+}
+
+// 16 bytes from a wave-uniform address and a lane's offset into LDS at
+// lds + 16 * lane (see lds_dma16 for why this is assembly)
+__device__ __forceinline__ void lds_load16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory");
+}
+
+template <class T, class O, int BM, int BN, int BK, int ST>
+__global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
+    constexpr int MI = BM / 64, NI = BN / 64;         // 32 x 32 blocks of a wave
+    constexpr int CH = BK / 8;                        // chunks of a row
+    constexpr int STAGE = (BM + BN) * BK * 2;         // bytes of a tile
+    constexpr int NL = (BM + BN) * CH / 256;          // loads of a thread for a tile
+    constexpr int PITCH = BN / 2 + 4;                 // floats of a row in the epilogue
+    static_assert(4 * 32 * PITCH * 4 <= ST * STAGE, "the epilogue's rows fit the buffers");
+    typedef typename Vec8<T>::type V;
+    __shared__ __align__(1024) unsigned char lds[ST * STAGE];
+    __shared__ __align__(16) float bias[BN];
+
+    // Workgroups go to the 8 XCDs in turn: each takes a run of tiles of its own,
+    // in columns of 8 tiles of rows, so that what its workgroups read at a time
+    // stays in its L2.
+    const uint32_t tiles = tiles_m * tiles_n, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
+    const uint32_t per = tiles / 8, more = tiles % 8;
+    const uint32_t tile = xcd * per + min(xcd, more) + nth;
+    const uint32_t group = tile / (8 * tiles_n), in = tile % (8 * tiles_n);
+    const uint32_t rows = min(8u, tiles_m - group * 8);
+    const uint64_t m0 = (uint64_t)(group * 8 + in % rows) * BM;
+    const uint32_t n0 = (in / rows) * BN;
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t lo = lane & 31, hi = lane >> 5;
+    for (uint32_t i = tid; i < BN; i += 256)
+        bias[i] = a.bias && n0 + i < a.n ? (float)((const T *)a.bias)[n0 + i] : 0.0f;
+
+    // this thread's chunks: rows 0..BM-1 are x's, BM.. are w's; rows past the
+    // end repeat the last one, their results are not stored
+    const char *xb = (const char *)((const T *)a.x + m0 * a.ldx), *wb = (const char *)((const T *)a.w + (uint64_t)n0 * a.ldw);
+    uint32_t off[NL], chunk[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const uint32_t idx = i * 256 + tid, row = idx / CH;
+        chunk[i] = (idx % CH) ^ swizzle<BK>(row);
+        off[i] = row < (uint32_t)BM ? (uint32_t)(min((uint64_t)row, a.m - 1 - m0) * a.ldx) * 2
+                                    : (uint32_t)(min(row - BM, a.n - 1 - n0) * a.ldw) * 2;
+    }
+    const uint32_t lds0 = lds_addr(lds) + wave * 1024;
+    const uint32_t steps = (a.k + BK - 1) / BK;
+    auto load = [&](uint32_t step) {
+        const uint32_t k0 = step * BK, buf = lds0 + step % ST * STAGE;
+        const bool part = k0 + BK > a.k;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            constexpr int XL = BM * CH / 256;
+            uint32_t c = chunk[i];
+            if (part) c = k0 + c * 8 < a.k ? c : 0;  // cleared below
+            lds_load16((i < XL ? xb : wb) + (uint64_t)k0 * 2, off[i] + c * 16, __builtin_amdgcn_readfirstlane(buf + i * 4096));
+        }
+    };
+
+    v16f acc[NI][MI];
+#pragma unroll
+    for (int n = 0; n < NI; n++)
+#pragma unroll
+        for (int m = 0; m < MI; m++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[n][m][e] = 0.0f;
+
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++)
+        if ((uint32_t)s < steps) load(s);
+    const uint32_t mrow = (wave & 1) * (BM / 2) + lo, nrow = BM + (wave >> 1) * (BN / 2) + lo;
+    for (uint32_t step = 0; step < steps; step++) {
+        if (step + ST - 1 <= steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 2) * NL));
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        unsigned char *buf = lds + step % ST * STAGE;
+        if (step + ST - 1 < steps) load(step + ST - 1);
+        if ((step + 1) * BK > a.k) {  // chunks past k: zeros in both operands
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                if (step * BK + chunk[i] * 8 >= a.k) *(v4i *)(buf + (i * 256 + tid) * 16) = v4i{0, 0, 0, 0};
+            __syncthreads();
+        }
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; kk++) {
+            V x[MI], w[NI];
+#pragma unroll
+            for (int m = 0; m < MI; m++) {
+                const uint32_t r = mrow + m * 32;
+                x[m] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
+            }
+#pragma unroll
+            for (int n = 0; n < NI; n++) {
+                const uint32_t r = nrow + n * 32;
+                w[n] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
+            }
+#pragma unroll
+            for (int n = 0; n < NI; n++)
+#pragma unroll
+                for (int m = 0; m < MI; m++) acc[n][m] = mfma32(w[n], x[m], acc[n][m]);
+        }
+    }
+    __syncthreads();
+
+    // Results by rows: 32 of a wave's rows at a time go through LDS as 32-bit
+    // floats, so that residuals are read and results written 16 bytes a lane
+    // along the rows.
+    float *rows32 = (float *)lds + wave * 32 * PITCH;
+    const uint32_t nw = (wave >> 1) * (BN / 2);
+#pragma unroll
+    for (int m = 0; m < MI; m++) {
+#pragma unroll
+        for (int n = 0; n < NI; n++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t col = n * 32 + q * 8 + hi * 4;
+                *(v4f *)(rows32 + lo * PITCH + col) =
+                    v4f{acc[n][m][q * 4], acc[n][m][q * 4 + 1], acc[n][m][q * 4 + 2], acc[n][m][q * 4 + 3]};
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own rows
+        const uint64_t mw = m0 + (wave & 1) * (BM / 2) + m * 32;
+#pragma unroll 2
+        for (int i = 0; i < 32 * BN / 2 / 8 / 64; i++) {
+            const uint32_t idx = i * 64 + lane, row = idx / (BN / 16), col = idx % (BN / 16) * 8;
+            float f[8];
+            *(v4f *)f = *(const v4f *)(rows32 + row * PITCH + col);
+            *(v4f *)(f + 4) = *(const v4f *)(rows32 + row * PITCH + col + 4);
+            float b[8];
+            *(v4f *)b = *(const v4f *)(bias + nw + col);
+            *(v4f *)(b + 4) = *(const v4f *)(bias + nw + col + 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] += b[e];
+            activate8(f, a.act);
+            if (mw + row < a.m && n0 + nw + col < a.n) finish8<O>(a, mw + row, n0 + nw + col, f);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// --------------------------------------------------------------- few rows --
+// Up to 16 * MF rows of x (one question, a few): w is read once, straight into
+// the matrix instructions' registers, 16 of its rows a workgroup; the waves
+// split k and join their sums in LDS.
+template <class T, class O, int MF>
+__global__ __launch_bounds__(1024) void linear_rows(LinearArgs a) {
+    typedef typename Vec8<T>::type V;
+    typedef typename Vec8<T>::unaligned VU;
+    extern __shared__ float red[];  // [wave][MF][256]
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const uint32_t n0 = blockIdx.x * 16, lo = lane & 15, kc = lane >> 4 << 3;
+    const T *w = (const T *)a.w + (uint64_t)min(n0 + lo, a.n - 1) * a.ldw + kc;
+    const T *x[MF];
+    v4f acc[MF];
+#pragma unroll
+    for (int m = 0; m < MF; m++) {
+        x[m] = (const T *)a.x + min((uint64_t)m * 16 + lo, a.m - 1) * a.ldx + kc;
+        acc[m] = v4f{0, 0, 0, 0};
+    }
+    const uint32_t steps = a.k / 32, each = (steps + waves - 1) / waves;
+    const uint32_t s0 = min(steps, wave * each), s1 = min(steps, s0 + each);
+#pragma unroll 4
+    for (uint32_t s = s0; s < s1; s++) {
+        const V wv = *(const VU *)(w + s * 32);
+#pragma unroll
+        for (int m = 0; m < MF; m++) acc[m] = mfma16(wv, (V) * (const VU *)(x[m] + s * 32), acc[m]);
+    }
+    if (steps * 32 < a.k && wave == waves - 1) {  // the rest of k, element by element
+        const uint32_t k = steps * 32, left = a.k - k;
+        V wv, xv;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const T e = w[kc + i < left ? (int)(k + i) : -(int)kc];
+            wv[i] = kc + i < left ? e : (T)0.0f;
+        }
+#pragma unroll
+        for (int m = 0; m < MF; m++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const T e = x[m][kc + i < left ? (int)(k + i) : -(int)kc];
+                xv[i] = kc + i < left ? e : (T)0.0f;
+            }
+            acc[m] = mfma16(wv, xv, acc[m]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MF; m++) *(v4f *)(red + (wave * MF + m) * 256 + lo * 16 + (lane >> 4) * 4) = acc[m];
+    __syncthreads();
+    // red[wave][row][column]: eight columns of a row a thread
+    for (uint32_t i = threadIdx.x; i < MF * 32; i += blockDim.x) {
+        float f[8] = {};
+        for (uint32_t v = 0; v < waves; v++) {
+            const v4f *r = (const v4f *)(red + v * MF * 256 + i * 8);
+            const v4f p = r[0], q = r[1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] += p[e], f[e + 4] += q[e];
+        }
+        const uint32_t row = i / 2, n = n0 + i % 2 * 8;
+        if (row >= a.m || n >= a.n) continue;
+        if (a.bias)
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] += (float)((const T *)a.bias)[min(n + e, a.n - 1)];
+        activate8(f, a.act);
+        finish8<O>(a, row, n, f);
+    }
+}
+
+// ---------------------------------------------------------------- packing --
+// Rows for linear_tile, which loads 16 bytes at 16-byte addresses: k rounded
+// up to 8 with zeros.
+template <class T>
+__global__ __launch_bounds__(256) void pack_rows(const T *x, uint64_t ldx, uint32_t k, uint32_t chunks, uint64_t count, T *y) {
+    const uint64_t step = (uint64_t)gridDim.x * 256;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += step) {
+        const uint64_t row = i / chunks;
+        const uint32_t at = (uint32_t)(i - row * chunks) * 8;
+        const T *p = x + row * ldx + at;
+        typename Vec8<T>::type v;
+        if (at + 8 <= k) {
+            v = *(const typename Vec8<T>::unaligned *)p;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const T z = p[at + e < k ? e : 0];
+                v[e] = at + e < k ? z : (T)0.0f;
+            }
+        }
+        *(typename Vec8<T>::type *)(y + i * 8) = v;
+    }
+}
+
+constexpr uint64_t FEW_ROWS = 64;
+
+bool aligned(const void *p, uint64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+bool packs(const LinearArgs &a, const void *p, uint64_t ld) {
+    return a.m > FEW_ROWS && a.k && (a.k % 8 || !aligned(p, ld) || ld >= (1u << 22));
+}
+uint64_t packed_bytes(uint64_t rows, uint32_t k) { return (rows * ((k + 7) / 8) * 16 + 255) & ~255ull; }
+
+template <class T>
+hipError_t pack(const void *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *to, hipStream_t s) {
+    const uint32_t chunks = (k + 7) / 8;
+    const uint64_t count = rows * chunks;
+    pack_rows<T><<<(uint32_t)std::min<uint64_t>((count + 255) / 256, 8192), 256, 0, s>>>((const T *)p, ld, k, chunks, count, (T *)to);
+    p = to;
+    ld = (uint64_t)chunks * 8;
+    return hipGetLastError();
+}
+
+template <class T, class O, int BM, int BN, int BK, int ST>
+hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
+    const uint32_t tn = (a.n + BN - 1) / BN;
+    // a launch holds fewer than 2^32 threads
+    const uint64_t most = std::max<uint64_t>(1, (1u << 23) / tn);
+    for (uint64_t m = 0; m < a.m; m += most * BM) {
+        LinearArgs b = a;
+        b.m = std::min(a.m - m, most * BM);
+        b.x = (const T *)a.x + m * a.ldx;
+        b.y = (O *)a.y + m * a.ldy;
+        if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
+        const uint32_t tm = (uint32_t)((b.m + BM - 1) / BM);
+        linear_tile<T, O, BM, BN, BK, ST><<<tm * tn, 256, 0, s>>>(b, tm, tn);
     }
     return hipGetLastError();
 }
 
+template <class T, class O, int MF>
+hipError_t rows_of(const LinearArgs &a, hipStream_t s) {
+    const uint32_t waves = a.k <= 512 ? 4 : a.k <= 1024 ? 8 : 16;
+    linear_rows<T, O, MF><<<(a.n + 15) / 16, waves * 64, waves * MF * 1024, s>>>(a);
+    return hipGetLastError();
+}
+
+template <class T, class O>
+hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
+    if (a.m <= FEW_ROWS) {
+        if (a.m <= 16) return rows_of<T, O, 1>(a, s);
+        if (a.m <= 32) return rows_of<T, O, 2>(a, s);
+        return rows_of<T, O, 4>(a, s);
+    }
+    const bool px = packs(a, a.x, a.ldx), pw = packs(a, a.w, a.ldw);
+    if (px) {
+        const hipError_t e = pack<T>(a.x, a.ldx, a.m, a.k, ws, s);
+        if (e != hipSuccess) return e;
+        ws = (char *)ws + packed_bytes(a.m, a.k);
+    }
+    if (pw) {
+        const hipError_t e = pack<T>(a.w, a.ldw, a.n, a.k, ws, s);
+        if (e != hipSuccess) return e;
+    }
+    const uint64_t big = ((a.m + 127) / 128) * ((a.n + 255) / 256), mid = ((a.m + 127) / 128) * ((a.n + 127) / 128);
+    if (a.k % 8) a.k = (a.k + 7) / 8 * 8;
+    if (big >= 512) return tile_of<T, O, 128, 256, 32, 3>(a, s);
+    if (mid >= 512) return tile_of<T, O, 128, 128, 64, 2>(a, s);
+    return tile_of<T, O, 64, 64, 64, 4>(a, s);
+}
+
 }  // namespace
 
-hipError_t launch_linear(const LinearArgs &a, hipStream_t s) {
-    if (a.dtype == T_F16) return a.out_dtype == T_F32 ? linear_of<f16, float>(a, s) : linear_of<f16, f16>(a, s);
-    return a.out_dtype == T_F32 ? linear_of<bf16, float>(a, s) : linear_of<bf16, bf16>(a, s);
+size_t linear_workspace(const LinearArgs &a) {
+    return (packs(a, a.x, a.ldx) ? packed_bytes(a.m, a.k) : 0) + (packs(a, a.w, a.ldw) ? packed_bytes(a.n, a.k) : 0);
+}
+
+hipError_t launch_linear(const LinearArgs &a, void *ws, hipStream_t s) {
+    if (a.dtype == T_F16) return a.out_dtype == T_F32 ? linear_of<f16, float>(a, ws, s) : linear_of<f16, f16>(a, ws, s);
+    return a.out_dtype == T_F32 ? linear_of<bf16, float>(a, ws, s) : linear_of<bf16, bf16>(a, ws, s);
 }
 
 }  // namespace bvk
