@@ -15,6 +15,7 @@ struct bv_embed {
     std::mutex mu;
     bv_device *dev = nullptr;
     hipStream_t own = nullptr, stream = nullptr;
+    void *zeros = nullptr;  // 256 bytes of zeros
     // Workspaces of each stream that needed one, the last of a stream's in
     // use.  Smaller ones stay until the handle goes, since captured graphs hold
     // their addresses; each is at least one and a half times the one before.
@@ -158,10 +159,15 @@ extern "C" int bv_embed_create(bv_device *dev, bv_embed **out) {
     bv_embed *e = new (std::nothrow) bv_embed();
     if (!e) return fail(BV_E_OOM, "out of host memory");
     e->dev = dev;
-    const hipError_t err = hipStreamCreateWithFlags(&e->own, hipStreamNonBlocking);
+    hipError_t err = hipStreamCreateWithFlags(&e->own, hipStreamNonBlocking);
+    if (err == hipSuccess) err = hipMalloc(&e->zeros, 256);
+    if (err == hipSuccess) err = hipMemset(e->zeros, 0, 256);
+    if (err == hipSuccess) err = hipStreamSynchronize(nullptr);  // before any stream's first call
     if (err != hipSuccess) {
+        if (e->zeros) (void)hipFree(e->zeros);
+        if (e->own) (void)hipStreamDestroy(e->own);
         delete e;
-        return hip_fail(dev, err, "hipStreamCreate");
+        return hip_fail(dev, err, "bv_embed_create");
     }
     e->stream = e->own;
     *out = e;
@@ -173,6 +179,7 @@ extern "C" int bv_embed_destroy(bv_embed *e) {
     (void)hipSetDevice(e->dev->ordinal);
     (void)hipDeviceSynchronize();
     for (const auto &w : e->ws) (void)hipFree(w.p);
+    (void)hipFree(e->zeros);
     (void)hipStreamDestroy(e->own);
     delete e;
     return BV_OK;
@@ -403,7 +410,10 @@ extern "C" int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *ar
     t.svh = a.v_head_stride;
     t.so = a.o_stride;
     t.soh = a.o_head_stride;
-    HIPX(e->dev, launch_attention(t, e->stream), "attention kernel");
+    t.zeros = e->zeros;
+    void *ws = nullptr;
+    OK_OR_RETURN(embed_workspace(e, attention_workspace(t), &ws));
+    HIPX(e->dev, launch_attention(t, ws, e->stream), "attention kernel");
     return BV_OK;
 }
 

@@ -33,8 +33,11 @@ struct AttentionArgs {
     void *o;
     const int32_t *cu_q, *cu_k;
     uint64_t sq, sqh, sk, skh, sv, svh, so, soh;  // token and head strides
+    const void *zeros;                            // 16 bytes of zeros
 };
-hipError_t launch_attention(const AttentionArgs &a, hipStream_t s);
+// Bytes of workspace that a call needs (partial results of split keys).
+size_t attention_workspace(const AttentionArgs &a);
+hipError_t launch_attention(const AttentionArgs &a, void *ws, hipStream_t s);
 
 // ------------------------------------------------------------------ rows --
 struct RotaryArgs {

@@ -235,7 +235,6 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own rows
         const uint64_t mw = m0 + (wave & 1) * (BM / 2) + m * 32;
-#pragma unroll 2
         for (int i = 0; i < 32 * BN / 2 / 8 / 64; i++) {
             const uint32_t idx = i * 64 + lane, row = idx / (BN / 16), col = idx % (BN / 16) * 8;
             float f[8];
