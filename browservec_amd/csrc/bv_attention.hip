@@ -31,12 +31,6 @@ __device__ __forceinline__ v16f mfma32(Vec8<bf16>::type a, Vec8<bf16>::type b, v
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// the other half's value: lane ^ 32
-__device__ __forceinline__ float other_half(float x) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
-
 // What a call's kernels share beside its arguments: the split of the keys and
 // where partial results go.
 struct AttentionPlan {
@@ -299,7 +293,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
             for (int k = 0; k < KB; k++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) best = fmaxf(best, s[k][b][e]);
-            best = fmaxf(best, other_half(best)) * pl.c;
+            best = halves_max(best) * pl.c;
             // The maximum that weights refer to follows when one passes it by
             // 2^8: until then weights stay below 2^8, and nothing is rescaled.
             if (__any(best > top[b] + 8.0f)) {
@@ -354,7 +348,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
     }
 #pragma unroll
     for (int b = 0; b < QB; b++) {
-        const float total = sum[b] + other_half(sum[b]);
+        const float total = halves_sum(sum[b]);
         if (wrow + b * 32 + lo >= p.rows) continue;
         if (pl.splits > 1) {
             const uint64_t at = ((uint64_t)split * a.tq + token[b]) * a.hq + head[b];
@@ -429,9 +423,9 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, Attention
 // The shape of a head dimension's tiles.
 template <int D>
 struct Shape {
-    static constexpr int QB = D <= 64 ? 2 : 1, KT = D <= 128 ? 64 : 32, ST = 2;
+    static constexpr int QB = 1, KT = D <= 128 ? 64 : 32, ST = 2;
 };
-uint32_t rows_of_tile(uint32_t d) { return d <= 64 ? 256 : 128; }
+uint32_t rows_of_tile(uint32_t d) { return 128; }
 uint32_t keys_of_tile(uint32_t d) { return d <= 128 ? 64 : 32; }
 
 // Parts of the keys: where tiles of rows alone leave most of the card idle, and

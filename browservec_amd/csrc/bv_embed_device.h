@@ -67,15 +67,42 @@ __device__ __forceinline__ void store8(T *p, int n, const float (&f)[8]) {
         if (i < n) p[i] = (T)f[i];
 }
 
+// Over the wave, the result in every lane, in the VALU alone: within rows of 16
+// lanes by permutations of quads and mirrors, across rows by swaps (a swap of x
+// with itself gives a lane its own value and its partner's).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+#define BV_OVER_WAVE(x, OP)                                                                              \
+    x = OP(x, dpp<0xb1>(x));  /* quads: 1 0 3 2 */                                                       \
+    x = OP(x, dpp<0x4e>(x));  /* quads: 2 3 0 1 */                                                       \
+    x = OP(x, dpp<0x141>(x)); /* halves of a row mirrored */                                             \
+    x = OP(x, dpp<0x140>(x)); /* rows mirrored */                                                        \
+    {                                                                                                    \
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false); \
+        x = OP(__uint_as_float(r[0]), __uint_as_float(r[1]));                                            \
+        r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);      \
+        x = OP(__uint_as_float(r[0]), __uint_as_float(r[1]));                                            \
+    }
+__device__ __forceinline__ float add_f32(float a, float b) { return a + b; }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    BV_OVER_WAVE(x, add_f32)
     return x;
 }
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    BV_OVER_WAVE(x, fmaxf)
     return x;
+}
+#undef BV_OVER_WAVE
+// A lane's value and that of lane ^ 32.
+__device__ __forceinline__ float halves_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float halves_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Packed sequences in tiles of `tile` places without a list of tiles: sequence

@@ -105,9 +105,10 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t s) {
 }
 
 // ----------------------------------------------------------------- norms --
-// A row in the registers of WAVES waves, CH chunks of eight elements a thread:
-// chunk j of thread i holds elements (j * 64 * WAVES + i) * 8 onwards, and
-// zeros past the row's end.
+// R rows in the registers of WAVES waves, CH chunks of eight elements a thread
+// and row: chunk j of thread i holds elements (j * 64 * WAVES + i) * 8 onwards,
+// and zeros past the row's end.  Several rows at a time: their loads are in
+// flight together and their reductions interleave.
 template <int WAVES>
 __device__ __forceinline__ float row_sum(float x, float *lds) {
     x = wave_sum(x);
@@ -121,39 +122,50 @@ __device__ __forceinline__ float row_sum(float x, float *lds) {
     return x;
 }
 
-// weights and biases: of any of the three types, loaded again for each row
-// (from the caches)
+// weights and biases: of any of the three types
 __device__ __forceinline__ void load8_of(int type, const void *p, uint32_t at, uint32_t n, bool tail, float (&f)[8]) {
     if (type == T_F32) load8((const float *)p, at, n, tail, f);
     else if (type == T_F16) load8((const f16 *)p, at, n, tail, f);
     else load8((const bf16 *)p, at, n, tail, f);
 }
 
-template <class T, int WAVES, int CH>
-__device__ __forceinline__ void normed_row(const NormArgs &a, const T *x, uint32_t i, float *lds, float (&f)[CH][8]) {
-    const bool tail = a.dim % 8 != 0;
+// What the norm does to each row: (f - mean) * r.
+template <int WAVES, int CH, int R>
+__device__ __forceinline__ void norm_stats(const NormArgs &a, uint32_t i, float *lds, const float (&f)[R][CH][8],
+                                           float (&mean)[R], float (&r)[R]) {
 #pragma unroll
-    for (int j = 0; j < CH; j++) load8(x, (j * 64 * WAVES + i) * 8, a.dim, tail, f[j]);
-    float mean = 0, r = 1;
+    for (int k = 0; k < R; k++) mean[k] = 0.0f, r[k] = 1.0f;
     if (a.norm == 1) {
-        float sum = 0;
+        float sum[R] = {};
 #pragma unroll
-        for (int j = 0; j < CH; j++)
+        for (int k = 0; k < R; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += f[j][e];
-        mean = row_sum<WAVES>(sum, lds) / (float)a.dim;
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum[k] += f[k][j][e];
+#pragma unroll
+        for (int k = 0; k < R; k++) mean[k] = row_sum<WAVES>(sum[k], lds) / (float)a.dim;
     }
     if (a.norm) {  // the squares about the mean, after it: no cancellation
-        float sq = 0;
+        float sq[R] = {};
 #pragma unroll
-        for (int j = 0; j < CH; j++)
+        for (int k = 0; k < R; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float d = (j * 64 * WAVES + i) * 8 + e < a.dim ? f[j][e] - mean : 0.0f;
-                sq = fmaf(d, d, sq);
-            }
-        r = 1.0f / sqrtf(row_sum<WAVES>(sq, lds) / (float)a.dim + a.eps);
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float d = (j * 64 * WAVES + i) * 8 + e < a.dim ? f[k][j][e] - mean[k] : 0.0f;
+                    sq[k] = fmaf(d, d, sq[k]);
+                }
+#pragma unroll
+        for (int k = 0; k < R; k++) r[k] = 1.0f / sqrtf(row_sum<WAVES>(sq[k], lds) / (float)a.dim + a.eps);
     }
+}
+
+// f times the weights plus the biases, zeros past the row's end.
+template <int WAVES, int CH, int R>
+__device__ __forceinline__ void weighted(const NormArgs &a, uint32_t i, float (&f)[R][CH][8]) {
+    const bool tail = a.dim % 8 != 0;
 #pragma unroll
     for (int j = 0; j < CH; j++) {
         const uint32_t at = (j * 64 * WAVES + i) * 8;
@@ -163,7 +175,9 @@ __device__ __forceinline__ void normed_row(const NormArgs &a, const T *x, uint32
         if (a.w) load8_of(a.wtype, a.w, at, a.dim, tail, w);
         if (a.b) load8_of(a.wtype, a.b, at, a.dim, tail, b);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[j][e] = at + e < a.dim ? fmaf((f[j][e] - mean) * r, w[e], b[e]) : 0.0f;
+        for (int k = 0; k < R; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[k][j][e] = at + e < a.dim ? fmaf(f[k][j][e], w[e], b[e]) : 0.0f;
     }
 }
 
@@ -190,33 +204,58 @@ __device__ __forceinline__ void store_row(const NormArgs &a, O *y, uint32_t i, f
     }
 }
 
-// One output row per WAVES waves: a token's (no pooling), or the first or last
-// of a sequence's.
-template <class T, class O, int WAVES, int CH>
+// R output rows per WAVES waves: tokens' (no pooling), or the first or last of
+// each sequence's.
+template <class T, class O, int WAVES, int CH, int R>
 __global__ __launch_bounds__(256) void norm_rows(NormArgs a, uint64_t first) {
     __shared__ float lds[4];
     const uint32_t i = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const uint64_t row = first + (WAVES == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
-    uint64_t from = row;
-    bool empty = false;
-    if (a.pool) {
-        if (row >= a.batch) return;
-        const int64_t b = clip_cu(a.cu, row, a.tokens), e = clip_cu(a.cu, row + 1, a.tokens);
-        empty = e <= b;
-        from = a.pool == 2 ? b : e - 1;
-    } else if (row >= a.tokens) {
-        return;
+    const uint64_t row0 = first + (WAVES == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x) * R;
+    const uint64_t rows = a.pool ? a.batch : a.tokens;
+    if (row0 >= rows) return;
+    const bool tail = a.dim % 8 != 0;
+    float f[R][CH][8];
+    bool empty[R];
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const uint64_t row = min(row0 + k, rows - 1);
+        int64_t from = row;
+        empty[k] = false;
+        if (a.pool) {
+            const int64_t b = clip_cu(a.cu, row, a.tokens), e = clip_cu(a.cu, row + 1, a.tokens);
+            empty[k] = e <= b;
+            from = empty[k] ? 0 : a.pool == 2 ? b : e - 1;
+        }
+        if (a.tokens == 0) {
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[k][j][e] = 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+                load8((const T *)a.x + from * a.ldx, (j * 64 * WAVES + i) * 8, a.dim, tail, f[k][j]);
+        }
     }
-    float f[CH][8];
-    if (empty) {
+    float mean[R], r[R];
+    norm_stats<WAVES, CH, R>(a, i, lds, f, mean, r);
+#pragma unroll
+    for (int k = 0; k < R; k++)
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[j][e] = 0.0f;
-    } else {
-        normed_row<T, WAVES, CH>(a, (const T *)a.x + from * a.ldx, i, lds, f);
+            for (int e = 0; e < 8; e++) f[k][j][e] = (f[k][j][e] - mean[k]) * r[k];
+    weighted<WAVES, CH, R>(a, i, f);
+    if (WAVES > 1) __syncthreads();  // y may be x: every thread has its elements
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        if (empty[k])
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[k][j][e] = 0.0f;
+        if (row0 + k < rows) store_row<O, WAVES, CH>(a, (O *)a.y + (row0 + k) * a.ldy, i, lds, f[k]);
     }
-    store_row<O, WAVES, CH>(a, (O *)a.y + row * a.ldy, i, lds, f);
 }
 
 // --------------------------------------------------------------- pooling --
@@ -224,11 +263,12 @@ __global__ __launch_bounds__(256) void norm_rows(NormArgs a, uint64_t first) {
 // sequence (its slot, see slot_sequence), waves taking rows in turn, and
 // writes a partial sum, or the result where the sequence has no more rows; a
 // second launch joins the partial sums of longer sequences in their order.
+// Weights and biases are applied to the mean: they are the same for every row.
 constexpr uint32_t POOL_CHUNK = 64;
 
-template <class T, int WAVES, int CH>
+template <class T, int WAVES, int CH, int R>
 __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
-    constexpr int ROWS = 4 / WAVES;  // rows at a time
+    constexpr int ROWS = 4 / WAVES;  // waves with rows of their own
     extern __shared__ float acc_lds[];
     __shared__ float lds[4];
     const uint64_t slot = first + blockIdx.x;
@@ -238,14 +278,23 @@ __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
     const int64_t r0 = b + chunk * POOL_CHUNK, r1 = min(e, r0 + POOL_CHUNK);
     if (chunk < 0 || (chunk && r0 >= e)) return;  // chunk 0 of an empty sequence writes its zeros
     const uint32_t i = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, wave = WAVES == 1 ? threadIdx.x >> 6 : 0;
-    float acc[CH][8] = {};
-    for (int64_t r = r0 + wave; r < r1; r += ROWS) {
-        float f[CH][8];
-        normed_row<T, WAVES, CH>(a, (const T *)a.x + r * a.ldx, i, lds, f);
+    const bool tail = a.dim % 8 != 0;
+    float acc[1][CH][8] = {};
+    for (int64_t row = r0 + wave * R; row < r1; row += ROWS * R) {
+        float f[R][CH][8], mean[R], r[R];
 #pragma unroll
-        for (int j = 0; j < CH; j++)
+        for (int k = 0; k < R; k++)
 #pragma unroll
-            for (int x = 0; x < 8; x++) acc[j][x] += f[j][x];
+            for (int j = 0; j < CH; j++)
+                load8((const T *)a.x + min(row + k, r1 - 1) * a.ldx, (j * 64 * WAVES + i) * 8, a.dim, tail, f[k][j]);
+        norm_stats<WAVES, CH, R>(a, i, lds, f, mean, r);
+#pragma unroll
+        for (int k = 0; k < R; k++)
+            if (row + k < r1)
+#pragma unroll
+                for (int j = 0; j < CH; j++)
+#pragma unroll
+                    for (int x = 0; x < 8; x++) acc[0][j][x] += (f[k][j][x] - mean[k]) * r[k];
     }
     if (ROWS > 1) {  // the waves' sums, by halves
         const uint32_t span = CH * 512;
@@ -254,13 +303,13 @@ __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
 #pragma unroll
                 for (int j = 0; j < CH; j++)
 #pragma unroll
-                    for (int x = 0; x < 8; x++) acc_lds[(wave - h) * span + (j * 8 + x) * 64 + i] = acc[j][x];
+                    for (int x = 0; x < 8; x++) acc_lds[(wave - h) * span + (j * 8 + x) * 64 + i] = acc[0][j][x];
             __syncthreads();
             if ((int)wave < h)
 #pragma unroll
                 for (int j = 0; j < CH; j++)
 #pragma unroll
-                    for (int x = 0; x < 8; x++) acc[j][x] += acc_lds[wave * span + (j * 8 + x) * 64 + i];
+                    for (int x = 0; x < 8; x++) acc[0][j][x] += acc_lds[wave * span + (j * 8 + x) * 64 + i];
             __syncthreads();
         }
         if (wave) return;
@@ -270,7 +319,7 @@ __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
             const uint32_t at = (j * 64 * WAVES + i) * 8;
-            if (at < a.dim) store8(p + at, (int)min(8u, a.dim - at), acc[j]);
+            if (at < a.dim) store8(p + at, (int)min(8u, a.dim - at), acc[0][j]);
         }
         return;
     }
@@ -278,8 +327,9 @@ __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
 #pragma unroll
     for (int j = 0; j < CH; j++)
 #pragma unroll
-        for (int x = 0; x < 8; x++) acc[j][x] *= inv;
-    store_row<float, WAVES, CH>(a, (float *)a.y + (uint64_t)s * a.ldy, i, lds, acc);
+        for (int x = 0; x < 8; x++) acc[0][j][x] *= inv;
+    if (e > b) weighted<WAVES, CH, 1>(a, i, acc);
+    store_row<float, WAVES, CH>(a, (float *)a.y + (uint64_t)s * a.ldy, i, lds, acc[0]);
 }
 
 template <int CH>
@@ -291,7 +341,7 @@ __global__ __launch_bounds__(256) void pool_join(NormArgs a, uint32_t first) {
     const uint32_t i = threadIdx.x;
     const uint64_t p0 = b / POOL_CHUNK + s;
     const uint32_t n = (uint32_t)((e - b + POOL_CHUNK - 1) / POOL_CHUNK);
-    float acc[CH][8] = {};
+    float acc[1][CH][8] = {};
     for (uint32_t c = 0; c < n; c++) {
         const float *p = a.part + (p0 + c) * a.dim;
 #pragma unroll
@@ -299,24 +349,25 @@ __global__ __launch_bounds__(256) void pool_join(NormArgs a, uint32_t first) {
             float f[8];
             load8(p, (j * 256 + i) * 8, a.dim, a.dim % 8 != 0, f);
 #pragma unroll
-            for (int x = 0; x < 8; x++) acc[j][x] += f[x];
+            for (int x = 0; x < 8; x++) acc[0][j][x] += f[x];
         }
     }
     const float inv = 1.0f / (float)(e - b);
 #pragma unroll
     for (int j = 0; j < CH; j++)
 #pragma unroll
-        for (int x = 0; x < 8; x++) acc[j][x] *= inv;
-    store_row<float, 4, CH>(a, (float *)a.y + (uint64_t)s * a.ldy, i, lds, acc);
+        for (int x = 0; x < 8; x++) acc[0][j][x] *= inv;
+    weighted<4, CH, 1>(a, i, acc);
+    store_row<float, 4, CH>(a, (float *)a.y + (uint64_t)s * a.ldy, i, lds, acc[0]);
 }
 
-template <class T, class O, int WAVES, int CH>
+template <class T, class O, int WAVES, int CH, int R>
 hipError_t norm_of(const NormArgs &a, hipStream_t s) {
     if (a.pool == 1) {
         const uint64_t chunks = pool_chunks(a.tokens, a.batch);
         const size_t lds = WAVES == 1 ? (size_t)2 * CH * 512 * 4 : 0;
         for (uint64_t c = 0; c < chunks; c += GRID_MOST)
-            pool_chunk<T, WAVES, CH><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c);
+            pool_chunk<T, WAVES, CH, R><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c);
         if (a.tokens <= POOL_CHUNK) return hipGetLastError();  // every sequence fits one chunk
         for (uint64_t b = 0; b < a.batch; b += GRID_MOST) {
             const uint32_t n = (uint32_t)std::min<uint64_t>(a.batch - b, GRID_MOST);
@@ -326,20 +377,21 @@ hipError_t norm_of(const NormArgs &a, hipStream_t s) {
         return hipGetLastError();
     }
     const uint64_t rows = a.pool ? a.batch : a.tokens;
-    for (uint64_t r = 0; r < rows; r += (uint64_t)GRID_MOST * (4 / WAVES)) {
-        const uint64_t blocks = WAVES == 1 ? (rows - r + 3) / 4 : rows - r;
-        norm_rows<T, O, WAVES, CH><<<(uint32_t)std::min<uint64_t>(blocks, GRID_MOST), 256, 0, s>>>(a, r);
+    constexpr uint64_t each = R * (4 / WAVES);
+    for (uint64_t r = 0; r < rows; r += GRID_MOST * each) {
+        const uint64_t blocks = (rows - r + each - 1) / each;
+        norm_rows<T, O, WAVES, CH, R><<<(uint32_t)std::min<uint64_t>(blocks, GRID_MOST), 256, 0, s>>>(a, r);
     }
     return hipGetLastError();
 }
 template <class T, class O>
 hipError_t norm_sized(const NormArgs &a, hipStream_t s) {
-    if (a.dim <= 512) return norm_of<T, O, 1, 1>(a, s);
-    if (a.dim <= 1024) return norm_of<T, O, 1, 2>(a, s);
-    if (a.dim <= 2048) return norm_of<T, O, 1, 4>(a, s);
-    if (a.dim <= 4096) return norm_of<T, O, 1, 8>(a, s);
-    if (a.dim <= 8192) return norm_of<T, O, 4, 4>(a, s);
-    return norm_of<T, O, 4, 8>(a, s);
+    if (a.dim <= 512) return norm_of<T, O, 1, 1, 2>(a, s);
+    if (a.dim <= 1024) return norm_of<T, O, 1, 2, 2>(a, s);
+    if (a.dim <= 2048) return norm_of<T, O, 1, 4, 2>(a, s);
+    if (a.dim <= 4096) return norm_of<T, O, 1, 8, 1>(a, s);
+    if (a.dim <= 8192) return norm_of<T, O, 4, 4, 1>(a, s);
+    return norm_of<T, O, 4, 8, 1>(a, s);
 }
 template <class T>
 hipError_t norm_typed(const NormArgs &a, hipStream_t s) {
