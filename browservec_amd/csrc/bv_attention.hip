@@ -157,18 +157,18 @@ __device__ __forceinline__ void row_alone(const AttentionArgs &a, const Attentio
     }
 }
 
-// QB blocks of 32 rows a wave, four waves; tiles of KT keys and values through
-// ST buffers in LDS, loaded straight into it where DIRECT (16-byte aligned rows
-// of whole chunks), through registers otherwise.  One barrier a tile: after a
-// wave's wait for its share of the oldest tile, and before the loads of the
-// next one go where the tile before was.
-template <class T, int D, int QB, int KT, int ST, bool DIRECT>
+// 32 rows a wave, four waves; keys and values in tiles of KT, two of each in
+// LDS, loaded straight into it where DIRECT (16-byte aligned rows of whole
+// chunks), through registers otherwise.  One barrier a tile: after a wave's
+// wait for its share of the tile, and before the next one's loads go where the
+// tile before was.  A wave's products and its softmax follow one another; the
+// matrix cores and the vector unit overlap between the SIMD's other waves.
+template <class T, int D, int KT, bool DIRECT>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl, uint64_t first) {
     typedef typename Vec8<T>::type V;
-    constexpr int CH = D / 8, NL = KT * CH / 256, KB = KT / 32, DB = D / 32;
-    constexpr int STAGE = 2 * KT * D * 2;
-    constexpr uint32_t ROWS = 128 * QB;
-    __shared__ __align__(1024) unsigned char lds[ST * STAGE];
+    constexpr int CH = D / 8, NL = KT * CH / 256, KB = KT / 32, DB = D / 32, TILE = KT * D * 2;
+    constexpr uint32_t ROWS = 128;
+    __shared__ __align__(1024) unsigned char lds[4 * TILE];  // keys, values, keys, values
     const uint32_t group = a.hq / a.hk, hk = blockIdx.y, split = blockIdx.z;
     Place p;
     if (!place_of(a, group, ROWS, first + gridDim.x - 1 - blockIdx.x, p)) return;
@@ -181,145 +181,152 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
     const int32_t per = ((p.lk + KT - 1) / KT + pl.splits - 1) / pl.splits;
     const int32_t t0 = split * per, t1 = min((seen_last + KT - 1) / KT, t0 + per);
 
-    // this wave's rows
-    const int64_t wrow = p.row0 + wave * 32 * QB, wend = min(p.rows, wrow + 32 * QB);
-    const bool works = wrow < p.rows;
-    const int32_t wave_all = works ? seen_by(a, p, (int32_t)(wrow / group)) : 0;          // every row sees these
-    const int32_t wave_any = works ? seen_by(a, p, (int32_t)((wend - 1) / group)) : 0;    // some row sees these
-    int32_t seen[QB];
-    int64_t token[QB], head[QB];
-    V q[QB][D / 16];
+    // this wave's rows, and the tiles that some of them see
+    const int64_t wrow = p.row0 + wave * 32, wend = min(p.rows, wrow + 32);
+    const int32_t wave_all = wrow < p.rows ? seen_by(a, p, (int32_t)(wrow / group)) : 0;
+    const int32_t wave_any = wrow < p.rows ? seen_by(a, p, (int32_t)((wend - 1) / group)) : 0;
+    const int32_t tw = min(t1, (wave_any + KT - 1) / KT);
     const T *zeros = (const T *)pl.zeros;
+    const int64_t row = wrow + lo;
+    const bool in = row < p.rows;
+    const int32_t query = in ? (int32_t)(row / group) : 0;
+    const int64_t token = p.qb + query, head = hk * group + (in ? row - (int64_t)query * group : 0);
+    const int32_t seen = in ? seen_by(a, p, query) : 0;
+    V q[D / 16];
 #pragma unroll
-    for (int b = 0; b < QB; b++) {
-        const int64_t row = wrow + b * 32 + lo;
-        const bool in = row < p.rows;
-        const int32_t query = in ? (int32_t)(row / group) : 0;
-        token[b] = p.qb + query;
-        head[b] = hk * group + (in ? row - (int64_t)query * group : 0);
-        seen[b] = in ? seen_by(a, p, query) : 0;
-        const T *src = (const T *)a.q + token[b] * a.sq + head[b] * a.sqh;
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-            q[b][i] = raw8(src, i * 16 + hi * 8, a.d, in, zeros);
-            if (pl.negate) q[b][i] = -q[b][i];
-        }
+    for (int i = 0; i < D / 16; i++) {
+        q[i] = raw8((const T *)a.q + token * a.sq + head * a.sqh, i * 16 + hi * 8, a.d, in, zeros);
+        if (pl.negate) q[i] = -q[i];
     }
 
-    const T *kp = (const T *)a.k + p.kb * a.sk + hk * a.skh, *vp = (const T *)a.v + p.kb * a.sv + hk * a.svh;
+    // A tile of keys or values to a place in LDS.  Rows past the last
+    // key repeat it: they get no weight, and a value that is not finite is looked
+    // for below.  Elements past d stay the zeros that the buffers begin with.
+    const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
+    const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
-    auto load = [&](int32_t t) {
-        const uint32_t buf = (uint32_t)(t - t0) % ST * STAGE;
+    // Where rows have a power of two of chunks, a thread's chunks of a tile lie at
+    // the same place of every 256 / CH-th row.
+    constexpr bool REGULAR = 256 % CH == 0;
+    const uint32_t r0 = tid / CH;
+    const uint32_t kc = ((tid % CH) ^ key_swizzle<D>(r0)) * 8, vc = ((tid % CH) ^ value_swizzle<D>(r0)) * 8;
+    const uint32_t koff = (r0 * (uint32_t)a.sk + kc) * 2, voff = (r0 * (uint32_t)a.sv + vc) * 2;
+    auto load = [&](int32_t t, uint32_t to, bool values) {
+        const uint64_t step = values ? a.sv : a.sk;
+        const char *base = (values ? vp : kp) + (uint64_t)t * KT * step * 2;
+        if (DIRECT && REGULAR && (t + 1) * KT <= p.lk) {
+            if ((values ? vc : kc) < a.d)
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+                    lds_load16(base + i * (256 / CH) * step * 2, values ? voff : koff,
+                               __builtin_amdgcn_readfirstlane(lds0 + to + i * 4096));
+            return;
+        }
+        const uint32_t last = p.lk - 1 - t * KT;
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const uint32_t idx = i * 256 + tid, row = idx / CH, slot = idx % CH;
-            const uint32_t kc = (slot ^ key_swizzle<D>(row)) * 8, vc = (slot ^ value_swizzle<D>(row)) * 8;
-            const int32_t j = t * KT + row;
-            const T *kr = kp + (int64_t)j * a.sk, *vr = vp + (int64_t)j * a.sv;
-            const bool in = j < p.lk;
+            const uint32_t idx = i * 256 + tid, r = idx / CH;
+            const uint32_t c = ((idx % CH) ^ (values ? value_swizzle<D>(r) : key_swizzle<D>(r))) * 8;
+            const uint32_t from = min(r, last);
             if (DIRECT) {
-                const T *ks = in && kc < a.d ? kr + kc : zeros, *vs = in && vc < a.d ? vr + vc : zeros;
-                lds_dma16(ks, __builtin_amdgcn_readfirstlane(lds0 + buf + i * 4096));
-                lds_dma16(vs, __builtin_amdgcn_readfirstlane(lds0 + buf + STAGE / 2 + i * 4096));
+                if (c < a.d)
+                    lds_load16(base, (from * (uint32_t)step + c) * 2,
+                               __builtin_amdgcn_readfirstlane(lds0 + to + i * 4096));
             } else {
-                *(V *)(lds + buf + idx * 16) = raw8(kr, kc, a.d, in, zeros);
-                *(V *)(lds + buf + STAGE / 2 + idx * 16) = raw8(vr, vc, a.d, in, zeros);
+                *(V *)(lds + to + idx * 16) = raw8((const T *)base + from * step, c, a.d, true, zeros);
             }
         }
     };
 
-    v16f o[DB][QB];
-    float top[QB], sum[QB];
+    v16f o[DB];
 #pragma unroll
-    for (int b = 0; b < QB; b++) {
-        top[b] = -INFINITY;
-        sum[b] = 0;
+    for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][b][e] = 0.0f;
-    }
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float top = -INFINITY, sum = 0;
     bool not_finite = false;
 
-#pragma unroll
-    for (int s = 0; s < ST - 1; s++)
-        if (t0 + s < t1) load(t0 + s);
-    for (int32_t t = t0; t < t1; t++) {
-        if (DIRECT) {
-            if (t + ST - 1 <= t1) __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 2) * 2 * NL));
-            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    // Values: 4 keys of 16 elements are read by 16 lanes and come back
+    // transposed, lane i with element i of the four keys.  Which eight keys a
+    // lane's half of an operand stands for is free as long as both operands
+    // agree: keys 4 hi + 0..3 and 8 + 4 hi + 0..3 of sixteen, as the scores lie.
+    const uint32_t vrow = hi * 4 + ((lane & 15) >> 2);
+    // chunk 2 i + hi of row lo: rows of a power of two of bytes take i * 32 by
+    // exclusive or, others (swizzled within four chunks) from two places
+    const uint32_t kat = lo * D * 2 + ((hi ^ key_swizzle<D>(lo)) << 4);
+    const uint32_t kat2 = lo * D * 2 + (((2 | hi) ^ key_swizzle<D>(lo)) << 4);
+    const uint32_t vat = TILE + vrow * D * 2 + ((((lane & 16) >> 3 | (lane & 2) >> 1) ^ value_swizzle<D>(vrow)) << 4) + (lane & 1) * 8;
+    if (t0 < t1) {
+        if (DIRECT && a.d < D) {  // what lies past d
+            for (uint32_t i = tid; i < 4 * TILE / 16; i += 256) *(v4i *)(lds + i * 16) = v4i{0, 0, 0, 0};
+            __syncthreads();
         }
+        load(t0, 0, false);
+        load(t0, TILE, true);
+    }
+    for (int32_t t = t0; t < t1; t++) {
+        const uint32_t at = ((uint32_t)(t - t0) & 1) * 2 * TILE;
+        if (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + ST - 1 < t1) load(t + ST - 1);
-        const unsigned char *kbuf = lds + (uint32_t)(t - t0) % ST * STAGE, *vbuf = kbuf + STAGE / 2;
-        if (a.causal && (t + 1) * KT > seen_first) {
+        if (t + 1 < t1) {
+            load(t + 1, 2 * TILE - at, false);
+            load(t + 1, 3 * TILE - at, true);
+        }
+        if ((t + 1) * KT > seen_first) {  // some rows do not see all of these values
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                not_finite |= any_not_finite(*(const v4i *)(vbuf + (i * 256 + tid) * 16), EXPONENT<T>);
+                not_finite |= any_not_finite(*(const v4i *)(lds + at + TILE + (i * 256 + tid) * 16), EXPONENT<T>);
         }
-        if (t * KT >= wave_any) continue;
+        if (t >= tw) continue;
 
-        v16f s[KB][QB];
+        v16f s[KB];
 #pragma unroll
         for (int k = 0; k < KB; k++) {
 #pragma unroll
-            for (int b = 0; b < QB; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[k][b][e] = 0.0f;
-            const uint32_t r = k * 32 + lo;
+            for (int e = 0; e < 16; e++) s[k][e] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                const V kv = *(const V *)(kbuf + r * D * 2 + (((i * 2 + hi) ^ key_swizzle<D>(r)) * 16));
-#pragma unroll
-                for (int b = 0; b < QB; b++) s[k][b] = mfma32(kv, q[b][i], s[k][b]);
+                const uint32_t from = D == 96 ? (i & 1 ? kat2 : kat) + at + i / 2 * 64 : (kat + at) ^ (i * 32);
+                s[k] = mfma32(*(const V *)(lds + from + k * 32 * D * 2), q[i], s[k]);
             }
         }
         if ((t + 1) * KT > wave_all) {
 #pragma unroll
             for (int k = 0; k < KB; k++)
 #pragma unroll
-                for (int b = 0; b < QB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int32_t j = t * KT + k * 32 + e / 4 * 8 + (int)hi * 4 + e % 4;
-                        s[k][b][e] = j < seen[b] ? s[k][b][e] : -INFINITY;
-                    }
-        }
-        V w[QB][KT / 16];
-#pragma unroll
-        for (int b = 0; b < QB; b++) {
-            float best = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < KB; k++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) best = fmaxf(best, s[k][b][e]);
-            best = halves_max(best) * pl.c;
-            // The maximum that weights refer to follows when one passes it by
-            // 2^8: until then weights stay below 2^8, and nothing is rescaled.
-            if (__any(best > top[b] + 8.0f)) {
-                const float next = fmaxf(top[b], best);
-                const float keep = top[b] == next ? 1.0f : __builtin_amdgcn_exp2f(top[b] - next);
-                top[b] = next;
-                sum[b] *= keep;
-#pragma unroll
-                for (int d = 0; d < DB; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][b][e] *= keep;
-            }
-            const float m = top[b] == -INFINITY ? 0.0f : top[b];
-#pragma unroll
-            for (int k = 0; k < KB; k++)
-#pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[k][b][e], pl.c, -m));
-                    sum[b] += x;
-                    w[b][k * 2 + e / 8][e % 8] = (T)x;
+                    const int32_t j = t * KT + k * 32 + e / 4 * 8 + (int)hi * 4 + e % 4;
+                    s[k][e] = j < seen ? s[k][e] : -INFINITY;
                 }
         }
-        // values: 4 keys of 16 elements are read by 16 lanes and come back
-        // transposed, lane i with element i of the four keys.  Which eight keys a
-        // lane's half of an operand stands for is free as long as both operands
-        // agree: keys 4 hi + 0..3 and 8 + 4 hi + 0..3 of sixteen, as the scores lie.
+        float best = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) best = fmaxf(best, s[k][e]);
+        best = halves_max(best) * pl.c;
+        // The maximum that weights refer to follows when one passes it by 2^8:
+        // until then weights stay below 2^8, and nothing is rescaled.
+        if (__any(best > top + 8.0f)) {
+            const float now = fmaxf(top, best);
+            const float keep = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= keep;
+        }
+        const float m = top == -INFINITY ? 0.0f : top;
+        V w[KT / 16];
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[k][e], pl.c, -m));
+                sum += x;
+                w[k * 2 + e / 8][e % 8] = (T)x;
+            }
 #pragma unroll
         for (int k = 0; k < KT / 16; k++)
 #pragma unroll
@@ -330,63 +337,57 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
                 } v;
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const uint32_t r = k * 16 + x * 8 + hi * 4 + ((lane & 15) >> 2);
-                    const uint32_t e = d * 32 + (lane & 16) + (lane & 3) * 4;
-                    const uint32_t at = r * D * 2 + (((e >> 3) ^ value_swizzle<D>(r)) * 16) + (e & 7) * 2;
-                    v.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vbuf + at));
+                    const uint32_t from = D % 64 == 0 ? (vat + at) ^ (d * 64) : vat + at + d * 64;
+                    v.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + from + (k * 16 + x * 8) * D * 2));
                 }
-#pragma unroll
-                for (int b = 0; b < QB; b++) o[d][b] = mfma32(v.all, w[b][k], o[d][b]);
+                o[d] = mfma32(v.all, w[k], o[d]);
             }
     }
 
     if (__syncthreads_or(not_finite)) {
         float *own = (float *)lds + wave * 320;
-        for (int64_t row = wrow; row < wend; row++)
-            row_alone<T>(a, pl, p, group, hk, row, t0 * KT, (t0 + per) * KT, split, own, own + 256);
+        for (int64_t i = wrow; i < wend; i++)
+            row_alone<T>(a, pl, p, group, hk, i, t0 * KT, (t0 + per) * KT, split, own, own + 256);
         return;
     }
-#pragma unroll
-    for (int b = 0; b < QB; b++) {
-        const float total = halves_sum(sum[b]);
-        if (wrow + b * 32 + lo >= p.rows) continue;
-        if (pl.splits > 1) {
-            const uint64_t at = ((uint64_t)split * a.tq + token[b]) * a.hq + head[b];
-            if (hi == 0) pl.part_ml[at] = make_float2(top[b], total);
-            if (t0 >= t1) continue;
-            float *out = pl.part_o + at * a.d;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const uint32_t i = d * 32 + e * 2 + hi * 4;
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        if (i + x < a.d) out[i + x] = o[d][b][e + x];
-                }
-            continue;
-        }
-        const float r = 1.0f / total;
-        T *out = (T *)a.o + token[b] * a.so + head[b] * a.soh;
+    const float total = halves_sum(sum);
+    if (!in) return;
+    if (pl.splits > 1) {
+        const uint64_t at = ((uint64_t)split * a.tq + token) * a.hq + head;
+        if (hi == 0) pl.part_ml[at] = make_float2(top, total);
+        if (t0 >= t1) return;
+        float *out = pl.part_o + at * a.d;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const uint32_t i = d * 32 + e * 2 + hi * 4;
-                typedef T V4 __attribute__((ext_vector_type(4)));
-                typedef V4 V4U __attribute__((aligned(sizeof(T))));
-                V4 f;
 #pragma unroll
-                for (int x = 0; x < 4; x++) f[x] = (T)(seen[b] > 0 ? o[d][b][e + x] * r : 0.0f);
-                if (i + 4 <= a.d) {
-                    *(V4U *)(out + i) = f;
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        if (i + x < a.d) out[i + x] = f[x];
-                }
+                for (int x = 0; x < 4; x++)
+                    if (i + x < a.d) out[i + x] = o[d][e + x];
             }
+        return;
     }
+    const float scale = 1.0f / total;
+    T *out = (T *)a.o + token * a.so + head * a.soh;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const uint32_t i = d * 32 + e * 2 + hi * 4;
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            typedef V4 V4U __attribute__((aligned(sizeof(T))));
+            V4 f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) f[x] = (T)(seen > 0 ? o[d][e + x] * scale : 0.0f);
+            if (i + 4 <= a.d) {
+                *(V4U *)(out + i) = f;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (i + x < a.d) out[i + x] = f[x];
+            }
+        }
 }
 
 // Joins the parts of a row, a wave each, in their order.
@@ -420,30 +421,24 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, Attention
         if (c * 64 + lane < a.d) o[c * 64 + lane] = (T)(seen_by(a, p, query) > 0 ? acc[c] / sum : 0.0f);
 }
 
-// The shape of a head dimension's tiles.
-template <int D>
-struct Shape {
-    static constexpr int QB = 1, KT = D <= 128 ? 64 : 32, ST = 2;
-};
-uint32_t rows_of_tile(uint32_t d) { return 128; }
-uint32_t keys_of_tile(uint32_t d) { return d <= 128 ? 64 : 32; }
+constexpr uint32_t TILE_ROWS = 128;
+constexpr uint32_t tile_keys(uint32_t d) { return d <= 128 ? 64 : 32; }
 
 // Parts of the keys: where tiles of rows alone leave most of the card idle, and
 // no more than tiles of keys.
 uint32_t splits_of(const AttentionArgs &a) {
-    const uint64_t tiles = (a.tq * (a.hq / a.hk) / rows_of_tile(a.d) + a.batch) * a.hk;
+    const uint64_t tiles = (a.tq * (a.hq / a.hk) / TILE_ROWS + a.batch) * a.hk;
     const uint64_t keys = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
-    const uint64_t most = (keys + 4 * keys_of_tile(a.d) - 1) / (4 * keys_of_tile(a.d));
+    const uint64_t most = (keys + 4 * tile_keys(a.d) - 1) / (4 * tile_keys(a.d));
     return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({512 / tiles, most, 256}));
 }
 
 template <class T, int D, bool DIRECT>
 hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    typedef Shape<D> S;
-    const uint64_t slots = a.tq * (a.hq / a.hk) / (128 * S::QB) + a.batch;
+    const uint64_t slots = a.tq * (a.hq / a.hk) / TILE_ROWS + a.batch;
     for (uint64_t f = 0; f < slots; f += 1u << 23) {
         const dim3 grid((uint32_t)std::min<uint64_t>(slots - f, 1u << 23), a.hk, pl.splits);
-        attention_tile<T, D, S::QB, S::KT, S::ST, DIRECT><<<grid, 256, 0, s>>>(a, pl, f);
+        attention_tile<T, D, tile_keys(D), DIRECT><<<grid, 256, 0, s>>>(a, pl, f);
     }
     if (pl.splits > 1) {
         const uint64_t rows = a.tq * (a.hq / a.hk) / 4 + a.batch;
@@ -455,7 +450,7 @@ hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipS
 
 template <class T>
 hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    const bool direct = a.d % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.sk | a.skh | a.sv | a.svh) % 8 == 0;
+    const bool direct = a.d % 8 == 0 && std::max(a.sk, a.sv) < (1u << 24) && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.sk | a.skh | a.sv | a.svh) % 8 == 0;
     if (!direct) {
         if (a.d <= 64) return attention_sized<T, 64, false>(a, pl, s);
         if (a.d <= 128) return attention_sized<T, 128, false>(a, pl, s);

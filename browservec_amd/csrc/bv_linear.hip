@@ -113,13 +113,6 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
     return BK == 64 ? row & 7 : (row >> 1) & 3;
 }
 
-// 16 bytes from a wave-uniform address and a lane's offset into LDS at
-// lds + 16 * lane (see lds_dma16 for why this is assembly)
-__device__ __forceinline__ void lds_load16(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-                 : "memory");
-}
-
 template <class T, class O, int BM, int BN, int BK, int ST>
 __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int MI = BM / 64, NI = BN / 64;         // 32 x 32 blocks of a wave

@@ -34,6 +34,11 @@ __device__ __forceinline__ void lds_dma16_nt(const void *src, uint32_t off, uint
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(src), "s"(lds)
                  : "memory");
 }
+// The same, kept in the caches.
+__device__ __forceinline__ void lds_load16(const void *src, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(src), "s"(lds)
+                 : "memory");
+}
 __device__ __forceinline__ void lds_dma4(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory");
 }
