@@ -65,16 +65,17 @@ __device__ __forceinline__ int32_t seen_by(const AttentionArgs &a, const Place &
 }
 
 // LDS rows of D elements in 16-byte chunks; chunk c of row r lies at
-// c ^ swizzle.  Keys: eight lanes read the same chunk of consecutive rows and
-// cover all banks.  Values: sixteen lanes read 32 bytes of four consecutive
-// rows (a transposing read), which cover all banks.
+// c ^ swizzle.  LDS serves 256 bytes a cycle.  Keys: sixteen lanes read the same
+// chunk of consecutive rows and cover all banks.  Values: 32 lanes read 64
+// bytes of four consecutive rows (a transposing read), which cover all banks.
+// (Swizzles that covered 128 bytes spent half of LDS's time on conflicts.)
 template <int D>
 __device__ __forceinline__ uint32_t key_swizzle(uint32_t row) {
-    return D % 64 == 0 ? row & 7 : (row >> 1) & 3;
+    return D % 128 == 0 ? row & 15 : D == 64 ? row >> 1 & 7 : row >> 2 & 3;
 }
 template <int D>
 __device__ __forceinline__ uint32_t value_swizzle(uint32_t row) {
-    return D % 64 == 0 ? (row & 3) << 1 : (row >> 1 & 1) << 1;
+    return D % 128 == 0 ? (row & 3) << 2 : D == 64 ? (row >> 1 & 1) << 2 : 0;
 }
 
 // Eight elements from at on of a row of d, zeros past its end, in the type
@@ -205,9 +206,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
     const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
     const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
-    // Where rows have a power of two of chunks, a thread's chunks of a tile lie at
-    // the same place of every 256 / CH-th row.
-    constexpr bool REGULAR = 256 % CH == 0;
+    // Where rows have 4, 8 or 16 chunks, a thread's chunks of a tile lie at the
+    // same place of every 256 / CH-th row.
+    constexpr bool REGULAR = 256 % CH == 0 && CH <= 16;
     const uint32_t r0 = tid / CH;
     const uint32_t kc = ((tid % CH) ^ key_swizzle<D>(r0)) * 8, vc = ((tid % CH) ^ value_swizzle<D>(r0)) * 8;
     const uint32_t koff = (r0 * (uint32_t)a.sk + kc) * 2, voff = (r0 * (uint32_t)a.sv + vc) * 2;

@@ -105,12 +105,12 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_
 // steps ahead and multiplies.
 //
 // LDS rows hold BK elements, in 16-byte chunks; chunk c of row r lies at
-// c ^ swizzle(r), so that eight lanes that read the same chunk of consecutive
-// rows cover all banks.  Loads put lane i's chunk at a fixed place, so the
+// c ^ swizzle(r), so that sixteen lanes that read the same chunk of consecutive
+// rows cover all banks (256 bytes).  Loads put lane i's chunk at a fixed place, so the
 // swizzle is applied to the address they load from.
 template <int BK>
 __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
-    return BK == 64 ? row & 7 : (row >> 1) & 3;
+    return BK == 64 ? row >> 1 & 7 : row >> 2 & 3;
 }
 
 template <class T, class O, int BM, int BN, int BK, int ST>
