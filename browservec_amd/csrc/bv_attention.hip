@@ -170,9 +170,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
     constexpr int CH = D / 8, NL = KT * CH / 256, KB = KT / 32, DB = D / 32, TILE = KT * D * 2;
     constexpr uint32_t ROWS = 128;
     __shared__ __align__(1024) unsigned char lds[4 * TILE];  // keys, values, keys, values
-    const uint32_t group = a.hq / a.hk, hk = blockIdx.y, split = blockIdx.z;
+    // The last tiles of rows first: with a causal mask they take longest.  Key
+    // heads side by side: workgroups that run together spread over them, and
+    // where 8 is a multiple of their number, an XCD reads those of one.
+    const uint32_t group = a.hq / a.hk, nth = blockIdx.x / a.hk, hk = blockIdx.x - nth * a.hk, split = blockIdx.z;
     Place p;
-    if (!place_of(a, group, ROWS, first + gridDim.x - 1 - blockIdx.x, p)) return;
+    if (!place_of(a, group, ROWS, first + gridDim.x / a.hk - 1 - nth, p)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lo = lane & 31, hi = lane >> 5;
 
@@ -437,8 +440,9 @@ uint32_t splits_of(const AttentionArgs &a) {
 template <class T, int D, bool DIRECT>
 hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
     const uint64_t slots = a.tq * (a.hq / a.hk) / TILE_ROWS + a.batch;
-    for (uint64_t f = 0; f < slots; f += 1u << 23) {
-        const dim3 grid((uint32_t)std::min<uint64_t>(slots - f, 1u << 23), a.hk, pl.splits);
+    const uint64_t most = std::max<uint64_t>(1, (1u << 23) / a.hk);  // a grid's dimension holds fewer than 2^32 threads
+    for (uint64_t f = 0; f < slots; f += most) {
+        const dim3 grid((uint32_t)std::min<uint64_t>(slots - f, most) * a.hk, 1, pl.splits);
         attention_tile<T, D, tile_keys(D), DIRECT><<<grid, 256, 0, s>>>(a, pl, f);
     }
     if (pl.splits > 1) {
