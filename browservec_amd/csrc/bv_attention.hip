@@ -158,17 +158,26 @@ __device__ __forceinline__ void row_alone(const AttentionArgs &a, const Attentio
     }
 }
 
-// 32 rows a wave, four waves; keys and values in tiles of KT, two of each in
-// LDS, loaded straight into it where DIRECT (16-byte aligned rows of whole
-// chunks), through registers otherwise.  One barrier a tile: after a wave's
-// wait for its share of the tile, and before the next one's loads go where the
-// tile before was.  A wave's products and its softmax follow one another; the
-// matrix cores and the vector unit overlap between the SIMD's other waves.
-template <class T, int D, int KT, bool DIRECT>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl, uint64_t first) {
+// 32 rows a wave; keys and values in tiles of KT, two of each in LDS, loaded
+// straight into it where DIRECT (16-byte aligned rows of whole chunks), through
+// registers otherwise.
+//
+// A tile takes a wave two phases: products (the values of the tile before and
+// the scores of this one; matrix cores) and softmax (vector unit).
+//   GROUPS 1: four waves, phase after phase, one barrier a tile.  What overlaps
+//     are the waves of other workgroups; four of them fit a CU up to D = 64.
+//   GROUPS 2: eight waves, two a SIMD, of which one multiplies while the other
+//     does its softmax, held apart by a barrier a phase.  (Two workgroups of
+//     GROUPS 1 that share a CU fall into step, both waves of a SIMD multiplying
+//     and then both computing weights: 2300 cycles a tile and wave at D = 128
+//     where the products take 1024.)
+template <class T, int D, int KT, int GROUPS, bool DIRECT>
+__global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
+                                                                                 uint64_t first) {
     typedef typename Vec8<T>::type V;
-    constexpr int CH = D / 8, NL = KT * CH / 256, KB = KT / 32, DB = D / 32, TILE = KT * D * 2;
-    constexpr uint32_t ROWS = 128;
+    constexpr int THREADS = 256 * GROUPS, CH = D / 8, CHUNKS = KT * CH, NL = (CHUNKS + THREADS - 1) / THREADS;
+    constexpr int KB = KT / 32, DB = D / 32, TILE = KT * D * 2;
+    constexpr uint32_t ROWS = 128 * GROUPS;
     __shared__ __align__(1024) unsigned char lds[4 * TILE];  // keys, values, keys, values
     // The last tiles of rows first: with a causal mask they take longest.  Key
     // heads side by side: workgroups that run together spread over them, and
@@ -203,15 +212,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
         if (pl.negate) q[i] = -q[i];
     }
 
-    // A tile of keys or values to a place in LDS.  Rows past the last
-    // key repeat it: they get no weight, and a value that is not finite is looked
-    // for below.  Elements past d stay the zeros that the buffers begin with.
+    // A tile of keys or values to a place in LDS.  Rows past the last key repeat
+    // it: they get no weight, and a value that is not finite is looked for
+    // below.  Elements past d stay the zeros that the buffers begin with.
     const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
     const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
     // Where rows have 4, 8 or 16 chunks, a thread's chunks of a tile lie at the
-    // same place of every 256 / CH-th row.
-    constexpr bool REGULAR = 256 % CH == 0 && CH <= 16;
+    // same place of every THREADS / CH-th row.
+    constexpr bool REGULAR = THREADS % CH == 0 && CHUNKS % THREADS == 0 && CH <= 16;
     const uint32_t r0 = tid / CH;
     const uint32_t kc = ((tid % CH) ^ key_swizzle<D>(r0)) * 8, vc = ((tid % CH) ^ value_swizzle<D>(r0)) * 8;
     const uint32_t koff = (r0 * (uint32_t)a.sk + kc) * 2, voff = (r0 * (uint32_t)a.sv + vc) * 2;
@@ -222,78 +231,131 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
             if ((values ? vc : kc) < a.d)
 #pragma unroll
                 for (int i = 0; i < NL; i++)
-                    lds_load16(base + i * (256 / CH) * step * 2, values ? voff : koff,
-                               __builtin_amdgcn_readfirstlane(lds0 + to + i * 4096));
+                    lds_load16(base + i * (THREADS / CH) * step * 2, values ? voff : koff,
+                               __builtin_amdgcn_readfirstlane(lds0 + to + i * THREADS * 16));
             return;
         }
         const uint32_t last = p.lk - 1 - t * KT;
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const uint32_t idx = i * 256 + tid, r = idx / CH;
+            if (CHUNKS % THREADS && i * THREADS + wave * 64 >= CHUNKS) break;
+            const uint32_t idx = i * THREADS + tid, r = idx / CH;
             const uint32_t c = ((idx % CH) ^ (values ? value_swizzle<D>(r) : key_swizzle<D>(r))) * 8;
             const uint32_t from = min(r, last);
             if (DIRECT) {
                 if (c < a.d)
                     lds_load16(base, (from * (uint32_t)step + c) * 2,
-                               __builtin_amdgcn_readfirstlane(lds0 + to + i * 4096));
+                               __builtin_amdgcn_readfirstlane(lds0 + to + i * THREADS * 16));
             } else {
                 *(V *)(lds + to + idx * 16) = raw8((const T *)base + from * step, c, a.d, true, zeros);
             }
         }
     };
+    auto wait_and_meet = [&] {  // this wave's loads have arrived, its reads are done
+        if (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto keys_at = [&](int32_t t) { return ((uint32_t)(t - t0) & 1) * 2 * TILE; };
 
-    v16f o[DB];
+    v16f o[DB], s[KB];
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    V w[KT / 16];
     float top = -INFINITY, sum = 0;
     bool not_finite = false;
 
-    // Values: 4 keys of 16 elements are read by 16 lanes and come back
-    // transposed, lane i with element i of the four keys.  Which eight keys a
-    // lane's half of an operand stands for is free as long as both operands
-    // agree: keys 4 hi + 0..3 and 8 + 4 hi + 0..3 of sixteen, as the scores lie.
+    // Both products read their operands from LDS a batch ahead of the matrix
+    // instructions that take them, in an order that the compiler is held to: left
+    // to itself it saves the registers and waits for every read.
+    //
+    // Tile t's weights times its values.  4 keys of 16 elements are read by 16
+    // lanes and come back transposed, lane i with element i of the four keys.
+    // Which eight keys a lane's half of an operand stands for is free as long as
+    // both operands agree: keys 4 hi + 0..3 and 8 + 4 hi + 0..3 of sixteen, as the
+    // scores lie.
     const uint32_t vrow = hi * 4 + ((lane & 15) >> 2);
-    // chunk 2 i + hi of row lo: rows of a power of two of bytes take i * 32 by
-    // exclusive or, others (swizzled within four chunks) from two places
-    const uint32_t kat = lo * D * 2 + ((hi ^ key_swizzle<D>(lo)) << 4);
-    const uint32_t kat2 = lo * D * 2 + (((2 | hi) ^ key_swizzle<D>(lo)) << 4);
     const uint32_t vat = TILE + vrow * D * 2 + ((((lane & 16) >> 3 | (lane & 2) >> 1) ^ value_swizzle<D>(vrow)) << 4) + (lane & 1) * 8;
-    if (t0 < t1) {
-        if (DIRECT && a.d < D) {  // what lies past d
-            for (uint32_t i = tid; i < 4 * TILE / 16; i += 256) *(v4i *)(lds + i * 16) = v4i{0, 0, 0, 0};
-            __syncthreads();
+    constexpr int VB = DB < 4 ? DB : 4, VBATCHES = KT / 16 * DB / VB;
+    auto read_values = [&](uint32_t at, int b, V(&v)[VB]) {
+        const int k = b * VB / DB;
+#pragma unroll
+        for (int i = 0; i < VB; i++) {
+            const int d = b * VB % DB + i;
+            union {
+                s16x4 half[2];
+                V all;
+            } u;
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t from = D % 64 == 0 ? (vat + at) ^ (d * 64) : vat + at + d * 64;
+                u.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + from + (k * 16 + x * 8) * D * 2));
+            }
+            v[i] = u.all;
         }
-        load(t0, 0, false);
-        load(t0, TILE, true);
-    }
-    for (int32_t t = t0; t < t1; t++) {
-        const uint32_t at = ((uint32_t)(t - t0) & 1) * 2 * TILE;
-        if (DIRECT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 1 < t1) {
-            load(t + 1, 2 * TILE - at, false);
-            load(t + 1, 3 * TILE - at, true);
-        }
+    };
+    auto weigh_values = [&](int32_t t) {
+        const uint32_t at = keys_at(t);
         if ((t + 1) * KT > seen_first) {  // some rows do not see all of these values
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                not_finite |= any_not_finite(*(const v4i *)(lds + at + TILE + (i * 256 + tid) * 16), EXPONENT<T>);
+                if (CHUNKS % THREADS == 0 || i * THREADS + wave * 64 < CHUNKS)
+                    not_finite |= any_not_finite(*(const v4i *)(lds + at + TILE + (i * THREADS + tid) * 16), EXPONENT<T>);
         }
-        if (t >= tw) continue;
-
-        v16f s[KB];
+        if (t >= tw) return;
+        V v[2][VB];
+        read_values(at, 0, v[0]);
 #pragma unroll
-        for (int k = 0; k < KB; k++) {
+        for (int b = 0; b < VBATCHES; b++) {
+            if (b + 1 < VBATCHES) read_values(at, b + 1, v[(b + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < VB; i++) {
+                const int d = b * VB % DB + i;
+                o[d] = mfma32(v[b & 1][i], w[b * VB / DB], o[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Scores of tile t.  Chunk 2 i + hi of row lo: rows of a power of two of bytes
+    // take i * 32 by exclusive or, others (swizzled within four chunks) from two
+    // places.
+    const uint32_t kat = lo * D * 2 + ((hi ^ key_swizzle<D>(lo)) << 4);
+    const uint32_t kat2 = lo * D * 2 + (((2 | hi) ^ key_swizzle<D>(lo)) << 4);
+    constexpr int BATCH = 4, BATCHES = KB * (D / 16) / BATCH;
+    auto read_keys = [&](uint32_t at, int b, V(&f)[BATCH]) {
+#pragma unroll
+        for (int x = 0; x < BATCH; x++) {
+            const int k = (b * BATCH + x) % KB, i = (b * BATCH + x) / KB;
+            const uint32_t from = D == 96 ? (i & 1 ? kat2 : kat) + at + i / 2 * 64 : (kat + at) ^ (i * 32);
+            f[x] = *(const V *)(lds + from + k * 32 * D * 2);
+        }
+    };
+    auto scores = [&](int32_t t) {
+        if (t >= tw) return;
+        const uint32_t at = keys_at(t);
+        V f[2][BATCH];
+        read_keys(at, 0, f[0]);
+#pragma unroll
+        for (int k = 0; k < KB; k++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[k][e] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const uint32_t from = D == 96 ? (i & 1 ? kat2 : kat) + at + i / 2 * 64 : (kat + at) ^ (i * 32);
-                s[k] = mfma32(*(const V *)(lds + from + k * 32 * D * 2), q[i], s[k]);
+        for (int b = 0; b < BATCHES; b++) {
+            if (b + 1 < BATCHES) read_keys(at, b + 1, f[(b + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const int k = (b * BATCH + i) % KB;  // neighbours do not wait for each other's sum
+                s[k] = mfma32(f[b & 1][i], q[(b * BATCH + i) / KB], s[k]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    // Scores to weights, after the values of the tiles before.
+    auto softmax = [&](int32_t t) {
+        if (t >= tw) return;
         if ((t + 1) * KT > wave_all) {
 #pragma unroll
             for (int k = 0; k < KB; k++)
@@ -322,7 +384,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
                 for (int e = 0; e < 16; e++) o[d][e] *= keep;
         }
         const float m = top == -INFINITY ? 0.0f : top;
-        V w[KT / 16];
 #pragma unroll
         for (int k = 0; k < KB; k++)
 #pragma unroll
@@ -331,21 +392,61 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tile(Attentio
                 sum += x;
                 w[k * 2 + e / 8][e % 8] = (T)x;
             }
+        if (GROUPS == 2)
 #pragma unroll
-        for (int k = 0; k < KT / 16; k++)
-#pragma unroll
-            for (int d = 0; d < DB; d++) {
-                union {
-                    s16x4 half[2];
-                    V all;
-                } v;
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint32_t from = D % 64 == 0 ? (vat + at) ^ (d * 64) : vat + at + d * 64;
-                    v.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + from + (k * 16 + x * 8) * D * 2));
-                }
-                o[d] = mfma32(v.all, w[k], o[d]);
+            for (int k = 0; k < KT / 16; k++) asm volatile("" : "+v"(w[k]));  // in this phase
+    };
+
+    if (t0 < t1) {
+        if (DIRECT && a.d < D) {  // what lies past d
+            for (uint32_t i = tid; i < 4 * TILE / 16; i += THREADS) *(v4i *)(lds + i * 16) = v4i{0, 0, 0, 0};
+            __syncthreads();
+        }
+        load(t0, 0, false);
+    }
+    if (GROUPS == 1) {
+        if (t0 < t1) load(t0, TILE, true);
+        for (int32_t t = t0; t < t1; t++) {
+            wait_and_meet();
+            if (t + 1 < t1) {
+                load(t + 1, keys_at(t + 1), false);
+                load(t + 1, keys_at(t + 1) + TILE, true);
             }
+            scores(t);
+            softmax(t);
+            weigh_values(t);
+        }
+    } else if (t0 < t1) {
+        // Phase 2 (t - t0) + g: group g multiplies for tile t, the next phase is its
+        // softmax.  At even phases everyone starts the loads of the next tile's
+        // keys and this one's values, which are waited for two phases later.
+        const uint32_t g = wave >> 2;
+        auto load_next = [&](int32_t t) {
+            if (t + 1 < t1) load(t + 1, keys_at(t + 1), false);
+            if (t < t1) load(t, keys_at(t) + TILE, true);
+        };
+        if (g) {
+            wait_and_meet();
+            load_next(t0);
+        }
+        for (int32_t t = t0; t <= t1; t++) {
+            if (g) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            } else {
+                wait_and_meet();
+                load_next(t);
+            }
+            if (t > t0) weigh_values(t - 1);
+            scores(t);
+            if (g) {
+                wait_and_meet();
+                load_next(t + 1);
+            } else {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            softmax(t);
+        }
+        if (!g) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
     if (__syncthreads_or(not_finite)) {
@@ -425,26 +526,32 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, Attention
         if (c * 64 + lane < a.d) o[c * 64 + lane] = (T)(seen_by(a, p, query) > 0 ? acc[c] / sum : 0.0f);
 }
 
-constexpr uint32_t TILE_ROWS = 128;
+constexpr int PAIRED = 96;
 constexpr uint32_t tile_keys(uint32_t d) { return d <= 128 ? 64 : 32; }
 
 // Parts of the keys: where tiles of rows alone leave most of the card idle, and
 // no more than tiles of keys.
 uint32_t splits_of(const AttentionArgs &a) {
-    const uint64_t tiles = (a.tq * (a.hq / a.hk) / TILE_ROWS + a.batch) * a.hk;
+    const uint64_t tiles = (a.tq * (a.hq / a.hk) / 128 + a.batch) * a.hk;
     const uint64_t keys = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
     const uint64_t most = (keys + 4 * tile_keys(a.d) - 1) / (4 * tile_keys(a.d));
     return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({512 / tiles, most, 256}));
 }
 
-template <class T, int D, bool DIRECT>
-hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    const uint64_t slots = a.tq * (a.hq / a.hk) / TILE_ROWS + a.batch;
-    const uint64_t most = std::max<uint64_t>(1, (1u << 23) / a.hk);  // a grid's dimension holds fewer than 2^32 threads
+template <class T, int D, int GROUPS, bool DIRECT>
+void launch_tiles(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
+    const uint64_t slots = a.tq * (a.hq / a.hk) / (128 * GROUPS) + a.batch;
+    const uint64_t most = std::max<uint64_t>(1, (1u << 22) / a.hk);  // a grid's dimension holds fewer than 2^32 threads
     for (uint64_t f = 0; f < slots; f += most) {
         const dim3 grid((uint32_t)std::min<uint64_t>(slots - f, most) * a.hk, 1, pl.splits);
-        attention_tile<T, D, tile_keys(D), DIRECT><<<grid, 256, 0, s>>>(a, pl, f);
+        attention_tile<T, D, tile_keys(D), GROUPS, DIRECT><<<grid, 256 * GROUPS, 0, s>>>(a, pl, f);
     }
+}
+
+template <class T, int D, bool DIRECT>
+hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
+    if (DIRECT && D >= PAIRED && a.tq * (a.hq / a.hk) / 256 * a.hk >= 256) launch_tiles<T, D, DIRECT ? 2 : 1, DIRECT>(a, pl, s);
+    else launch_tiles<T, D, 1, DIRECT>(a, pl, s);
     if (pl.splits > 1) {
         const uint64_t rows = a.tq * (a.hq / a.hk) / 4 + a.batch;
         for (uint64_t f = 0; f < rows; f += 1u << 23)
