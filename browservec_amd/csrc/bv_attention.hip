@@ -526,8 +526,10 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, Attention
         if (c * 64 + lane < a.d) o[c * 64 + lane] = (T)(seen_by(a, p, query) > 0 ? acc[c] / sum : 0.0f);
 }
 
-constexpr int PAIRED = 96;
-constexpr uint32_t tile_keys(uint32_t d) { return d <= 128 ? 64 : 32; }
+// Keys of a tile: what two of keys and two of values leave of LDS and what a
+// wave's scores leave of its registers.  With turns between products and softmax
+// 128 keys a phase beat 64 by 3 to 5% (D = 128).
+constexpr uint32_t tile_keys(uint32_t d, uint32_t groups = 1) { return d > 128 ? 32 : groups == 2 && d >= 96 ? 128 : 64; }
 
 // Parts of the keys: where tiles of rows alone leave most of the card idle, and
 // no more than tiles of keys.
@@ -544,13 +546,17 @@ void launch_tiles(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s
     const uint64_t most = std::max<uint64_t>(1, (1u << 22) / a.hk);  // a grid's dimension holds fewer than 2^32 threads
     for (uint64_t f = 0; f < slots; f += most) {
         const dim3 grid((uint32_t)std::min<uint64_t>(slots - f, most) * a.hk, 1, pl.splits);
-        attention_tile<T, D, tile_keys(D), GROUPS, DIRECT><<<grid, 256 * GROUPS, 0, s>>>(a, pl, f);
+        attention_tile<T, D, tile_keys(D, GROUPS), GROUPS, DIRECT><<<grid, 256 * GROUPS, 0, s>>>(a, pl, f);
     }
 }
 
 template <class T, int D, bool DIRECT>
 hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    if (DIRECT && D >= PAIRED && a.tq * (a.hq / a.hk) / 256 * a.hk >= 256) launch_tiles<T, D, DIRECT ? 2 : 1, DIRECT>(a, pl, s);
+    // Turns pay where the products are as long as the softmax (D >= 96) and the
+    // larger tiles of rows still fill the card: 16384 x 8 x 128 966 us against
+    // 1028, D = 96 393 against 434, but D = 64 1250 against 1158.
+    if (DIRECT && D >= 96 && a.tq * (a.hq / a.hk) / 256 * a.hk >= 256)
+        launch_tiles<T, D, DIRECT && D >= 96 ? 2 : 1, DIRECT>(a, pl, s);
     else launch_tiles<T, D, 1, DIRECT>(a, pl, s);
     if (pl.splits > 1) {
         const uint64_t rows = a.tq * (a.hq / a.hk) / 4 + a.batch;
