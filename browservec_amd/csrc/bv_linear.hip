@@ -97,12 +97,14 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_
 }
 
 // ------------------------------------------------------------------ tiles --
-// A workgroup of four waves computes BM x BN results, its waves a quarter
-// each (BM/2 x BN/2).  Tiles of BK columns of x and w stream through ST buffers
-// in LDS, loaded straight into it: in every step a wave waits for its share of
-// the oldest tile, meets the others at a barrier (which also says that the
-// buffer of the step before is free), starts the loads of the tile ST - 1
-// steps ahead and multiplies.
+// A workgroup of 2 x WN waves computes BM x BN results, a wave BM/2 x BN/WN of
+// them.  Tiles of BK columns of x and w stream through ST buffers
+// in LDS, loaded straight into it.  A wave reads the operands of 16 columns
+// while it multiplies those of the 16 before.  Before it multiplies a tile's
+// last 16, already in registers, it waits for its share of the next tile and
+// meets the others at a barrier: the next tile's first operands can then be
+// read, and the tile's buffer takes the tile ST steps ahead, while the matrix
+// cores are busy.
 //
 // LDS rows hold BK elements, in 16-byte chunks; chunk c of row r lies at
 // c ^ swizzle(r), so that sixteen lanes that read the same chunk of consecutive
@@ -113,14 +115,16 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
     return BK == 64 ? row >> 1 & 7 : row >> 2 & 3;
 }
 
-template <class T, class O, int BM, int BN, int BK, int ST>
-__global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t tiles_m, uint32_t tiles_n) {
-    constexpr int MI = BM / 64, NI = BN / 64;         // 32 x 32 blocks of a wave
+template <class T, class O, int BM, int BN, int WN, int BK, int ST>
+__global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear_tile(LinearArgs a, uint32_t tiles_m,
+                                                                                      uint32_t tiles_n) {
+    constexpr int THREADS = 128 * WN, WB = BN / WN;   // 2 x WN waves, of WB columns each
+    constexpr int MI = BM / 64, NI = WB / 32;         // 32 x 32 blocks of a wave
     constexpr int CH = BK / 8;                        // chunks of a row
     constexpr int STAGE = (BM + BN) * BK * 2;         // bytes of a tile
-    constexpr int NL = (BM + BN) * CH / 256;          // loads of a thread for a tile
-    constexpr int PITCH = BN / 2 + 4;                 // floats of a row in the epilogue
-    static_assert(4 * 32 * PITCH * 4 <= ST * STAGE, "the epilogue's rows fit the buffers");
+    constexpr int NL = (BM + BN) * CH / THREADS;        // loads of a thread for a tile
+    constexpr int PITCH = WB + 4;                     // floats of a row in the epilogue
+    static_assert(2 * WN * 32 * PITCH * 4 <= ST * STAGE, "the epilogue's rows fit the buffers");
     typedef typename Vec8<T>::type V;
     __shared__ __align__(1024) unsigned char lds[ST * STAGE];
     __shared__ __align__(16) float bias[BN];
@@ -138,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lo = lane & 31, hi = lane >> 5;
-    for (uint32_t i = tid; i < BN; i += 256)
+    for (uint32_t i = tid; i < BN; i += THREADS)
         bias[i] = a.bias && n0 + i < a.n ? (float)((const T *)a.bias)[n0 + i] : 0.0f;
 
     // this thread's chunks: rows 0..BM-1 are x's, BM.. are w's; rows past the
@@ -147,23 +151,23 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
     uint32_t off[NL], chunk[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-        const uint32_t idx = i * 256 + tid, row = idx / CH;
+        const uint32_t idx = i * THREADS + tid, row = idx / CH;
         chunk[i] = (idx % CH) ^ swizzle<BK>(row);
         off[i] = row < (uint32_t)BM ? (uint32_t)(min((uint64_t)row, a.m - 1 - m0) * a.ldx) * 2
                                     : (uint32_t)(min(row - BM, a.n - 1 - n0) * a.ldw) * 2;
     }
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
     const uint32_t steps = (a.k + BK - 1) / BK;
-    auto load = [&](uint32_t step) {
+    auto load_one = [&](uint32_t step, int i) {
+        constexpr int XL = BM * CH / THREADS;
         const uint32_t k0 = step * BK, buf = lds0 + step % ST * STAGE;
-        const bool part = k0 + BK > a.k;
+        uint32_t c = chunk[i];
+        if (k0 + BK > a.k) c = k0 + c * 8 < a.k ? c : 0;  // cleared in arrive()
+        lds_load16((i < XL ? xb : wb) + (uint64_t)k0 * 2, off[i] + c * 16, __builtin_amdgcn_readfirstlane(buf + i * THREADS * 16));
+    };
+    auto load = [&](uint32_t step) {
 #pragma unroll
-        for (int i = 0; i < NL; i++) {
-            constexpr int XL = BM * CH / 256;
-            uint32_t c = chunk[i];
-            if (part) c = k0 + c * 8 < a.k ? c : 0;  // cleared below
-            lds_load16((i < XL ? xb : wb) + (uint64_t)k0 * 2, off[i] + c * 16, __builtin_amdgcn_readfirstlane(buf + i * 4096));
-        }
+        for (int i = 0; i < NL; i++) load_one(step, i);
     };
 
     v16f acc[NI][MI];
@@ -174,39 +178,66 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[n][m][e] = 0.0f;
 
+    const uint32_t mrow = (wave & 1) * (BM / 2) + lo, nrow = BM + (wave >> 1) * WB + lo;
+    constexpr int KK = BK / 16;
+    V x[2][MI], w[2][NI];
+    auto read = [&](uint32_t step, int kk, V(&xs)[MI], V(&ws)[NI]) {
+        const unsigned char *buf = lds + step % ST * STAGE;
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++)
-        if ((uint32_t)s < steps) load(s);
-    const uint32_t mrow = (wave & 1) * (BM / 2) + lo, nrow = BM + (wave >> 1) * (BN / 2) + lo;
-    for (uint32_t step = 0; step < steps; step++) {
-        if (step + ST - 1 <= steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 2) * NL));
+        for (int n = 0; n < NI; n++) {
+            const uint32_t r = nrow + n * 32;
+            ws[n] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
+        }
+#pragma unroll
+        for (int m = 0; m < MI; m++) {
+            const uint32_t r = mrow + m * 32;
+            xs[m] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
+        }
+    };
+    // tile `step` is in LDS, for every wave
+    auto arrive = [&](uint32_t step) {
+        if (step + ST - 2 < steps) __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 2) * NL));
         else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        unsigned char *buf = lds + step % ST * STAGE;
-        if (step + ST - 1 < steps) load(step + ST - 1);
         if ((step + 1) * BK > a.k) {  // chunks past k: zeros in both operands
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                if (step * BK + chunk[i] * 8 >= a.k) *(v4i *)(buf + (i * 256 + tid) * 16) = v4i{0, 0, 0, 0};
+                if (step * BK + chunk[i] * 8 >= a.k)
+                    *(v4i *)(lds + step % ST * STAGE + (i * THREADS + tid) * 16) = v4i{0, 0, 0, 0};
             __syncthreads();
         }
+    };
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; kk++) {
-            V x[MI], w[NI];
+    for (int s = 0; s < ST - 1; s++)
+        if ((uint32_t)s < steps) load(s);
+    if (steps) {
+        arrive(0);
+        if (ST - 1 < steps) load(ST - 1);
+        read(0, 0, x[0], w[0]);
+    }
+    for (uint32_t step = 0; step < steps; step++) {
 #pragma unroll
-            for (int m = 0; m < MI; m++) {
-                const uint32_t r = mrow + m * 32;
-                x[m] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
+        for (int kk = 0; kk < KK; kk++) {
+            if (kk + 1 < KK) {
+                read(step, kk + 1, x[(kk + 1) & 1], w[(kk + 1) & 1]);
+            } else if (step + 1 < steps) {
+                arrive(step + 1);
+                read(step + 1, 0, x[0], w[0]);
             }
-#pragma unroll
-            for (int n = 0; n < NI; n++) {
-                const uint32_t r = nrow + n * 32;
-                w[n] = *(const V *)(buf + r * BK * 2 + (((kk * 2 + hi) ^ swizzle<BK>(r)) * 16));
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool loads = kk + 1 == KK && step + ST < steps;
 #pragma unroll
             for (int n = 0; n < NI; n++)
 #pragma unroll
-                for (int m = 0; m < MI; m++) acc[n][m] = mfma32(w[n], x[m], acc[n][m]);
+                for (int m = 0; m < MI; m++) {
+                    acc[n][m] = mfma32(w[kk & 1][n], x[kk & 1][m], acc[n][m]);
+                    constexpr int EACH = (NL + MI * NI - 1) / (MI * NI);
+                    if (loads)  // between matrix instructions, where issue is idle
+#pragma unroll
+                        for (int i = 0; i < EACH; i++)
+                            if ((n * MI + m) * EACH + i < NL) load_one(step + ST, (n * MI + m) * EACH + i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         }
     }
     __syncthreads();
@@ -215,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
     // floats, so that residuals are read and results written 16 bytes a lane
     // along the rows.
     float *rows32 = (float *)lds + wave * 32 * PITCH;
-    const uint32_t nw = (wave >> 1) * (BN / 2);
+    const uint32_t nw = (wave >> 1) * WB;
 #pragma unroll
     for (int m = 0; m < MI; m++) {
 #pragma unroll
@@ -228,8 +259,8 @@ __global__ __launch_bounds__(256, 2) void linear_tile(LinearArgs a, uint32_t til
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own rows
         const uint64_t mw = m0 + (wave & 1) * (BM / 2) + m * 32;
-        for (int i = 0; i < 32 * BN / 2 / 8 / 64; i++) {
-            const uint32_t idx = i * 64 + lane, row = idx / (BN / 16), col = idx % (BN / 16) * 8;
+        for (int i = 0; i < 32 * WB / 8 / 64; i++) {
+            const uint32_t idx = i * 64 + lane, row = idx / (WB / 8), col = idx % (WB / 8) * 8;
             float f[8];
             *(v4f *)f = *(const v4f *)(rows32 + row * PITCH + col);
             *(v4f *)(f + 4) = *(const v4f *)(rows32 + row * PITCH + col + 4);
@@ -354,11 +385,11 @@ hipError_t pack(const void *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *t
     return hipGetLastError();
 }
 
-template <class T, class O, int BM, int BN, int BK, int ST>
+template <class T, class O, int BM, int BN, int WN, int BK, int ST>
 hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
     const uint32_t tn = (a.n + BN - 1) / BN;
     // a launch holds fewer than 2^32 threads
-    const uint64_t most = std::max<uint64_t>(1, (1u << 23) / tn);
+    const uint64_t most = std::max<uint64_t>(1, (1u << 22) / tn);
     for (uint64_t m = 0; m < a.m; m += most * BM) {
         LinearArgs b = a;
         b.m = std::min(a.m - m, most * BM);
@@ -366,7 +397,7 @@ hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
         b.y = (O *)a.y + m * a.ldy;
         if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
         const uint32_t tm = (uint32_t)((b.m + BM - 1) / BM);
-        linear_tile<T, O, BM, BN, BK, ST><<<tm * tn, 256, 0, s>>>(b, tm, tn);
+        linear_tile<T, O, BM, BN, WN, BK, ST><<<tm * tn, 128 * WN, 0, s>>>(b, tm, tn);
     }
     return hipGetLastError();
 }
@@ -397,9 +428,9 @@ hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
     }
     const uint64_t big = ((a.m + 127) / 128) * ((a.n + 255) / 256), mid = ((a.m + 127) / 128) * ((a.n + 127) / 128);
     if (a.k % 8) a.k = (a.k + 7) / 8 * 8;
-    if (big >= 512) return tile_of<T, O, 128, 256, 32, 3>(a, s);
-    if (mid >= 512) return tile_of<T, O, 128, 128, 64, 2>(a, s);
-    return tile_of<T, O, 64, 64, 64, 4>(a, s);
+    if (big >= 512) return tile_of<T, O, 256, 256, 4, 64, 2>(a, s);
+    if (mid >= 512) return tile_of<T, O, 128, 128, 2, 64, 2>(a, s);
+    return tile_of<T, O, 64, 64, 2, 64, 4>(a, s);
 }
 
 }  // namespace
