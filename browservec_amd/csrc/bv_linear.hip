@@ -148,22 +148,23 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
     // this thread's chunks: rows 0..BM-1 are x's, BM.. are w's; rows past the
     // end repeat the last one, their results are not stored
     const char *xb = (const char *)((const T *)a.x + m0 * a.ldx), *wb = (const char *)((const T *)a.w + (uint64_t)n0 * a.ldw);
-    uint32_t off[NL], chunk[NL];
+    auto chunk = [&](int i) { return (i * THREADS + tid) % CH ^ swizzle<BK>((i * THREADS + tid) / CH); };
+    uint32_t off[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-        const uint32_t idx = i * THREADS + tid, row = idx / CH;
-        chunk[i] = (idx % CH) ^ swizzle<BK>(row);
-        off[i] = row < (uint32_t)BM ? (uint32_t)(min((uint64_t)row, a.m - 1 - m0) * a.ldx) * 2
-                                    : (uint32_t)(min(row - BM, a.n - 1 - n0) * a.ldw) * 2;
+        const uint32_t row = (i * THREADS + tid) / CH;
+        off[i] = (row < (uint32_t)BM ? (uint32_t)(min((uint64_t)row, a.m - 1 - m0) * a.ldx)
+                                     : (uint32_t)(min(row - BM, a.n - 1 - n0) * a.ldw)) * 2 + chunk(i) * 16;
     }
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
     const uint32_t steps = (a.k + BK - 1) / BK;
     auto load_one = [&](uint32_t step, int i) {
         constexpr int XL = BM * CH / THREADS;
-        const uint32_t k0 = step * BK, buf = lds0 + step % ST * STAGE;
-        uint32_t c = chunk[i];
-        if (k0 + BK > a.k) c = k0 + c * 8 < a.k ? c : 0;  // cleared in arrive()
-        lds_load16((i < XL ? xb : wb) + (uint64_t)k0 * 2, off[i] + c * 16, __builtin_amdgcn_readfirstlane(buf + i * THREADS * 16));
+        const uint32_t k0 = step * BK;
+        const char *base = (i < XL ? xb : wb) + (uint64_t)k0 * 2;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + step % ST * STAGE + i * THREADS * 16);
+        if (k0 + BK <= a.k) lds_load16(base, off[i], to);
+        else lds_load16(base, k0 + chunk(i) * 8 < a.k ? off[i] : off[i] - chunk(i) * 16, to);  // cleared in arrive()
     };
     auto load = [&](uint32_t step) {
 #pragma unroll
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
         if ((step + 1) * BK > a.k) {  // chunks past k: zeros in both operands
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                if (step * BK + chunk[i] * 8 >= a.k)
+                if (step * BK + chunk(i) * 8 >= a.k)
                     *(v4i *)(lds + step % ST * STAGE + (i * THREADS + tid) * 16) = v4i{0, 0, 0, 0};
             __syncthreads();
         }
