@@ -98,7 +98,8 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_
 
 // ------------------------------------------------------------------ tiles --
 // A workgroup of 2 x WN waves computes BM x BN results, a wave BM/2 x BN/WN of
-// them.  Tiles of BK columns of x and w stream through ST buffers
+// them; KG such groups share the columns of every tile and join their sums at
+// the end, where tiles are few and what counts is the number of steps.  Tiles of BK columns of x and w stream through ST buffers
 // in LDS, loaded straight into it.  A wave reads the operands of 16 columns
 // while it multiplies those of the 16 before.  Before it multiplies a tile's
 // last 16, already in registers, it waits for its share of the next tile and
@@ -112,19 +113,20 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_
 // swizzle is applied to the address they load from.
 template <int BK>
 __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
-    return BK == 64 ? row >> 1 & 7 : row >> 2 & 3;
+    return BK >= 128 ? row & 15 : BK == 64 ? row >> 1 & 7 : row >> 2 & 3;
 }
 
-template <class T, class O, int BM, int BN, int WN, int BK, int ST>
-__global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear_tile(LinearArgs a, uint32_t tiles_m,
-                                                                                      uint32_t tiles_n) {
-    constexpr int THREADS = 128 * WN, WB = BN / WN;   // 2 x WN waves, of WB columns each
+template <class T, class O, int BM, int BN, int WN, int BK, int ST, int KG = 1>
+__global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void linear_tile(LinearArgs a, uint32_t tiles_m,
+                                                                                           uint32_t tiles_n) {
+    constexpr int THREADS = 128 * WN * KG, WB = BN / WN;  // KG times 2 x WN waves, of WB columns each
     constexpr int MI = BM / 64, NI = WB / 32;         // 32 x 32 blocks of a wave
     constexpr int CH = BK / 8;                        // chunks of a row
     constexpr int STAGE = (BM + BN) * BK * 2;         // bytes of a tile
     constexpr int NL = (BM + BN) * CH / THREADS;        // loads of a thread for a tile
     constexpr int PITCH = WB + 4;                     // floats of a row in the epilogue
-    static_assert(2 * WN * 32 * PITCH * 4 <= ST * STAGE, "the epilogue's rows fit the buffers");
+    constexpr int ROWS_END = 2 * WN * 32 * PITCH * 4;  // bytes of those rows; after them, the other groups' sums
+    static_assert(ROWS_END + (KG - 1) * 2 * WN * MI * NI * 4096 <= ST * STAGE, "the epilogue's data fits the buffers");
     typedef typename Vec8<T>::type V;
     __shared__ __align__(1024) unsigned char lds[ST * STAGE];
     __shared__ __align__(16) float bias[BN];
@@ -140,7 +142,8 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
     const uint64_t m0 = (uint64_t)(group * 8 + in % rows) * BM;
     const uint32_t n0 = (in / rows) * BN;
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t tid = threadIdx.x, lane = tid & 63, any_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t wave = any_wave % (2 * WN), kg = any_wave / (2 * WN);
     const uint32_t lo = lane & 31, hi = lane >> 5;
     for (uint32_t i = tid; i < BN; i += THREADS)
         bias[i] = a.bias && n0 + i < a.n ? (float)((const T *)a.bias)[n0 + i] : 0.0f;
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
         off[i] = (row < (uint32_t)BM ? (uint32_t)(min((uint64_t)row, a.m - 1 - m0) * a.ldx)
                                      : (uint32_t)(min(row - BM, a.n - 1 - n0) * a.ldw)) * 2 + chunk(i) * 16;
     }
-    const uint32_t lds0 = lds_addr(lds) + wave * 1024;
+    const uint32_t lds0 = lds_addr(lds) + any_wave * 1024;
     const uint32_t steps = (a.k + BK - 1) / BK;
     auto load_one = [&](uint32_t step, int i) {
         constexpr int XL = BM * CH / THREADS;
@@ -180,9 +183,10 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
             for (int e = 0; e < 16; e++) acc[n][m][e] = 0.0f;
 
     const uint32_t mrow = (wave & 1) * (BM / 2) + lo, nrow = BM + (wave >> 1) * WB + lo;
-    constexpr int KK = BK / 16;
+    constexpr int KK = BK / 16 / KG;  // of a tile, for each group
     V x[2][MI], w[2][NI];
-    auto read = [&](uint32_t step, int kk, V(&xs)[MI], V(&ws)[NI]) {
+    auto read = [&](uint32_t step, int k, V(&xs)[MI], V(&ws)[NI]) {
+        const uint32_t kk = kg * KK + k;
         const unsigned char *buf = lds + step % ST * STAGE;
 #pragma unroll
         for (int n = 0; n < NI; n++) {
@@ -242,6 +246,26 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
         }
     }
     __syncthreads();
+    if (KG > 1) {  // the groups' sums, in their order
+        float *sums = (float *)(lds + ROWS_END) + (wave * 64 + lane) * 4;
+        constexpr int QUADS = MI * NI * 4, GROUP = 2 * WN * 64 * 4;  // floats from a quad to the next
+        if (kg)
+#pragma unroll
+            for (int i = 0; i < QUADS; i++) {
+                const v16f &f = acc[i / 4 / MI][i / 4 % MI];
+                *(v4f *)(sums + ((kg - 1) * QUADS + i) * GROUP) = v4f{f[i % 4 * 4], f[i % 4 * 4 + 1], f[i % 4 * 4 + 2], f[i % 4 * 4 + 3]};
+            }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; g++)
+#pragma unroll
+            for (int i = 0; i < QUADS; i++) {
+                const v4f f = *(const v4f *)(sums + (g * QUADS + i) * GROUP);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i / 4 / MI][i / 4 % MI][i % 4 * 4 + e] += f[e];
+            }
+    }
 
     // Results by rows: 32 of a wave's rows at a time go through LDS as 32-bit
     // floats, so that residuals are read and results written 16 bytes a lane
@@ -281,12 +305,14 @@ __global__ __launch_bounds__(128 * WN, BM * BN / WN > 16384 ? 1 : 2) void linear
 // Up to 16 * MF rows of x (one question, a few): w is read once, straight into
 // the matrix instructions' registers, 16 of its rows a workgroup; the waves
 // split k and join their sums in LDS.
+constexpr uint32_t ROW_WAVES = 8;
 template <class T, class O, int MF>
-__global__ __launch_bounds__(1024) void linear_rows(LinearArgs a) {
+__global__ __launch_bounds__(ROW_WAVES * 64) void linear_rows(LinearArgs a) {
     typedef typename Vec8<T>::type V;
     typedef typename Vec8<T>::unaligned VU;
-    extern __shared__ float red[];  // [wave][MF][256]
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    constexpr uint32_t waves = ROW_WAVES;
+    __shared__ __align__(16) float red[waves * MF * 256];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n0 = blockIdx.x * 16, lo = lane & 15, kc = lane >> 4 << 3;
     const T *w = (const T *)a.w + (uint64_t)min(n0 + lo, a.n - 1) * a.ldw + kc;
     const T *x[MF];
@@ -326,7 +352,7 @@ __global__ __launch_bounds__(1024) void linear_rows(LinearArgs a) {
     for (int m = 0; m < MF; m++) *(v4f *)(red + (wave * MF + m) * 256 + lo * 16 + (lane >> 4) * 4) = acc[m];
     __syncthreads();
     // red[wave][row][column]: eight columns of a row a thread
-    for (uint32_t i = threadIdx.x; i < MF * 32; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < MF * 32; i += waves * 64) {
         float f[8] = {};
         for (uint32_t v = 0; v < waves; v++) {
             const v4f *r = (const v4f *)(red + v * MF * 256 + i * 8);
@@ -368,7 +394,9 @@ __global__ __launch_bounds__(256) void pack_rows(const T *x, uint64_t ldx, uint3
     }
 }
 
-constexpr uint64_t FEW_ROWS = 64;
+// Rows up to which w goes straight to the registers: 32 rows, 4096 x 4096: 15.8
+// us, by tiles 17.7; 64 rows 21.7 and 19.2.
+constexpr uint64_t FEW_ROWS = 32;
 
 bool aligned(const void *p, uint64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
 bool packs(const LinearArgs &a, const void *p, uint64_t ld) {
@@ -386,7 +414,7 @@ hipError_t pack(const void *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *t
     return hipGetLastError();
 }
 
-template <class T, class O, int BM, int BN, int WN, int BK, int ST>
+template <class T, class O, int BM, int BN, int WN, int BK, int ST, int KG = 1>
 hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
     const uint32_t tn = (a.n + BN - 1) / BN;
     // a launch holds fewer than 2^32 threads
@@ -398,15 +426,15 @@ hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
         b.y = (O *)a.y + m * a.ldy;
         if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
         const uint32_t tm = (uint32_t)((b.m + BM - 1) / BM);
-        linear_tile<T, O, BM, BN, WN, BK, ST><<<tm * tn, 128 * WN, 0, s>>>(b, tm, tn);
+        linear_tile<T, O, BM, BN, WN, BK, ST, KG><<<tm * tn, 128 * WN * KG, 0, s>>>(b, tm, tn);
     }
     return hipGetLastError();
 }
 
 template <class T, class O, int MF>
 hipError_t rows_of(const LinearArgs &a, hipStream_t s) {
-    const uint32_t waves = a.k <= 512 ? 4 : a.k <= 1024 ? 8 : 16;
-    linear_rows<T, O, MF><<<(a.n + 15) / 16, waves * 64, waves * MF * 1024, s>>>(a);
+    // 8 waves: k 384 to 4096 within 0.1 us of the best of 4, 8 and 16
+    linear_rows<T, O, MF><<<(a.n + 15) / 16, ROW_WAVES * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -414,8 +442,7 @@ template <class T, class O>
 hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
     if (a.m <= FEW_ROWS) {
         if (a.m <= 16) return rows_of<T, O, 1>(a, s);
-        if (a.m <= 32) return rows_of<T, O, 2>(a, s);
-        return rows_of<T, O, 4>(a, s);
+        return rows_of<T, O, 2>(a, s);
     }
     const bool px = packs(a, a.x, a.ldx), pw = packs(a, a.w, a.ldw);
     if (px) {
@@ -427,11 +454,31 @@ hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
         const hipError_t e = pack<T>(a.w, a.ldw, a.n, a.k, ws, s);
         if (e != hipSuccess) return e;
     }
-    const uint64_t big = ((a.m + 127) / 128) * ((a.n + 255) / 256), mid = ((a.m + 127) / 128) * ((a.n + 127) / 128);
     if (a.k % 8) a.k = (a.k + 7) / 8 * 8;
-    if (big >= 512) return tile_of<T, O, 256, 256, 4, 64, 2>(a, s);
-    if (mid >= 512) return tile_of<T, O, 128, 128, 2, 64, 2>(a, s);
-    return tile_of<T, O, 64, 64, 2, 64, 4>(a, s);
+    // The shape that is done first: rounds of the tiles that the card holds at a
+    // time, each a + b k long (ns, fitted to 100..32768 x 384..8192 x 384..8192).
+    // 2037 x 768 x 768 (k 768): 8.6 us in the first, 11.2 in the second, 14.2 and
+    // 24.4 in the others; 4096 x 768: 14.7, 11.9, 14.7, 25.1; 8192 x 768: 23.4, 20.7,
+    // 18.5, 26.5; 16384 x 768: 42.9, 34.0, 31.3, 28.2.
+    struct {
+        uint32_t bm, bn, at_a_time, a, b;
+    } const shapes[4] = {{64, 64, 512, 2400, 73}, {128, 128, 256, 4700, 94}, {128, 128, 512, 3600, 174}, {256, 256, 256, 9800, 198}};
+    int best = 0;
+    uint64_t least = ~0ull;
+    for (int i = 0; i < 4; i++) {
+        const auto &t = shapes[i];
+        const uint64_t tiles = ((a.m + t.bm - 1) / t.bm) * ((a.n + t.bn - 1) / t.bn);
+        const uint64_t ns = (tiles + t.at_a_time - 1) / t.at_a_time * (t.a + (uint64_t)t.b * a.k / 10);
+        if (ns < least) least = ns, best = i;
+    }
+    switch (best) {
+    case 0:  // four groups where a CU has one tile (300 x 384, k 1536: 8.1 us against 9.5)
+        if (a.k >= 1024 && ((a.m + 63) / 64) * ((a.n + 63) / 64) <= 256) return tile_of<T, O, 64, 64, 2, 256, 2, 4>(a, s);
+        return tile_of<T, O, 64, 64, 2, 128, 2, 2>(a, s);
+    case 1: return tile_of<T, O, 128, 128, 4, 64, 4>(a, s);
+    case 2: return tile_of<T, O, 128, 128, 2, 64, 2>(a, s);
+    default: return tile_of<T, O, 256, 256, 4, 64, 2>(a, s);
+    }
 }
 
 }  // namespace
