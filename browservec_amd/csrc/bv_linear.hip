@@ -324,8 +324,21 @@ __global__ __launch_bounds__(ROW_WAVES * 64) void linear_rows(LinearArgs a) {
     }
     const uint32_t steps = a.k / 32, each = (steps + waves - 1) / waves;
     const uint32_t s0 = min(steps, wave * each), s1 = min(steps, s0 + each);
-#pragma unroll 4
-    for (uint32_t s = s0; s < s1; s++) {
+    uint32_t s = s0;
+    for (; s + 4 <= s1; s += 4) {  // four steps' loads in flight
+        V wv[4], xv[4][MF];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            wv[i] = *(const VU *)(w + (s + i) * 32);
+#pragma unroll
+            for (int m = 0; m < MF; m++) xv[i][m] = *(const VU *)(x[m] + (s + i) * 32);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int m = 0; m < MF; m++) acc[m] = mfma16(wv[i], xv[i][m], acc[m]);
+    }
+    for (; s < s1; s++) {
         const V wv = *(const VU *)(w + s * 32);
 #pragma unroll
         for (int m = 0; m < MF; m++) acc[m] = mfma16(wv, (V) * (const VU *)(x[m] + s * 32), acc[m]);
