@@ -36,7 +36,8 @@ __device__ __forceinline__ v16f mfma32(Vec8<bf16>::type a, Vec8<bf16>::type b, v
 struct AttentionPlan {
     float c;          // |scale| * log2(e): weights are powers of two
     int negate;       // scale < 0: the queries are negated
-    uint32_t splits;  // parts of every sequence's keys, each a workgroup's
+    uint32_t splits;  // parts of every sequence's keys, each a workgroup's or wave's
+    uint32_t chunk;   // keys of a part, whole tiles; the last part takes the rest
     float *part_o;    // [split][query][head][d], not yet divided by the sum
     float2 *part_ml;  // [split][query][head]: maximum (log2) and sum
     const void *zeros;  // 16 bytes of zeros that loads past an end read
@@ -62,6 +63,14 @@ __device__ __forceinline__ bool place_of(const AttentionArgs &a, uint32_t group,
 // How many of the sequence's keys a query sees: the first ones.
 __device__ __forceinline__ int32_t seen_by(const AttentionArgs &a, const Place &p, int32_t query) {
     return a.causal ? max(0, min(p.lk, p.lk - p.lq + query + 1)) : p.lk;
+}
+
+// The tiles of KT keys of a part: t0 up to the result.
+template <int KT>
+__device__ __forceinline__ int32_t part_of(const AttentionPlan &pl, uint32_t split, int32_t keys, int32_t &t0) {
+    const int32_t tiles = (keys + KT - 1) / KT, each = pl.chunk / KT;
+    t0 = (int32_t)min((int64_t)split * each, (int64_t)tiles);
+    return split + 1 == pl.splits ? tiles : min(tiles, t0 + each);
 }
 
 // LDS rows of D elements in 16-byte chunks; chunk c of row r lies at
@@ -158,6 +167,53 @@ __device__ __forceinline__ void row_alone(const AttentionArgs &a, const Attentio
     }
 }
 
+// A wave's 32 rows: the result, or a part of it that attention_join takes up
+// (any: it saw keys).
+template <class T, int D>
+__device__ __forceinline__ void store_rows(const AttentionArgs &a, const AttentionPlan &pl, const v16f (&o)[D / 32],
+                                           float top, float sum, bool in, int32_t seen, int64_t token, int64_t head,
+                                           uint32_t split, bool any) {
+    const uint32_t hi = (threadIdx.x & 63) >> 5;
+    const float total = halves_sum(sum);
+    if (!in) return;
+    if (pl.splits > 1) {
+        const uint64_t at = ((uint64_t)split * a.tq + token) * a.hq + head;
+        if (hi == 0) pl.part_ml[at] = make_float2(top, total);
+        if (!any) return;
+        float *out = pl.part_o + at * a.d;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t i = d * 32 + e * 2 + hi * 4;
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (i + x < a.d) out[i + x] = o[d][e + x];
+            }
+        return;
+    }
+    const float scale = 1.0f / total;
+    T *out = (T *)a.o + token * a.so + head * a.soh;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const uint32_t i = d * 32 + e * 2 + hi * 4;
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            typedef V4 V4U __attribute__((aligned(sizeof(T))));
+            V4 f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) f[x] = (T)(seen > 0 ? o[d][e + x] * scale : 0.0f);
+            if (i + 4 <= a.d) {
+                *(V4U *)(out + i) = f;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (i + x < a.d) out[i + x] = f[x];
+            }
+        }
+}
+
 // 32 rows a wave; keys and values in tiles of KT, two of each in LDS, loaded
 // straight into it where DIRECT (16-byte aligned rows of whole chunks), through
 // registers otherwise.
@@ -191,8 +247,8 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     const int64_t row_end = min(p.rows, p.row0 + ROWS);
     const int32_t seen_first = seen_by(a, p, (int32_t)(p.row0 / group));
     const int32_t seen_last = seen_by(a, p, (int32_t)((row_end - 1) / group));
-    const int32_t per = ((p.lk + KT - 1) / KT + pl.splits - 1) / pl.splits;
-    const int32_t t0 = split * per, t1 = min((seen_last + KT - 1) / KT, t0 + per);
+    int32_t t0;
+    const int32_t t1 = part_of<KT>(pl, split, seen_last, t0);
 
     // this wave's rows, and the tiles that some of them see
     const int64_t wrow = p.row0 + wave * 32, wend = min(p.rows, wrow + 32);
@@ -452,92 +508,244 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     if (__syncthreads_or(not_finite)) {
         float *own = (float *)lds + wave * 320;
         for (int64_t i = wrow; i < wend; i++)
-            row_alone<T>(a, pl, p, group, hk, i, t0 * KT, (t0 + per) * KT, split, own, own + 256);
+            row_alone<T>(a, pl, p, group, hk, i, t0 * KT, t1 * KT, split, own, own + 256);
         return;
     }
-    const float total = halves_sum(sum);
-    if (!in) return;
-    if (pl.splits > 1) {
-        const uint64_t at = ((uint64_t)split * a.tq + token) * a.hq + head;
-        if (hi == 0) pl.part_ml[at] = make_float2(top, total);
-        if (t0 >= t1) return;
-        float *out = pl.part_o + at * a.d;
+    store_rows<T, D>(a, pl, o, top, sum, in, seen, token, head, split, t0 < t1);
+}
+
+// Few rows a sequence (the next tokens over kept keys): what counts is to
+// stream keys and values.  Each wave works alone: 32 rows of one key head over
+// its part of the keys, 32 at a time through two tiles of its own in LDS, one on
+// its way; no barriers.  Neighbouring waves take the key heads side
+// by side in memory.
+template <class T, int D>
+__global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, AttentionPlan pl, uint64_t first, uint64_t units) {
+    typedef typename Vec8<T>::type V;
+    constexpr int KT = 32, CH = D / 8, NL = KT * CH / 64, DB = D / 32, TILE = KT * D * 2, ST = 2;
+    __shared__ __align__(1024) unsigned char all_lds[4 * ST * 2 * TILE];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lo = lane & 31, hi = lane >> 5;
+    unsigned char *lds = all_lds + wave * ST * 2 * TILE;
+    // unit: key head, then part of the keys, then tile of rows
+    const uint64_t unit = first + (uint64_t)blockIdx.x * 4 + wave;
+    if (unit >= units) return;
+    const uint32_t group = a.hq / a.hk, hk = (uint32_t)(unit % a.hk), split = (uint32_t)(unit / a.hk % pl.splits);
+    Place p;
+    if (!place_of(a, group, 32, unit / a.hk / pl.splits, p)) return;
+    const int64_t row = p.row0 + lo, wend = min(p.rows, p.row0 + 32);
+    const int32_t all = seen_by(a, p, (int32_t)(p.row0 / group)), any = seen_by(a, p, (int32_t)((wend - 1) / group));
+    int32_t t0;
+    const int32_t t1 = part_of<KT>(pl, split, any, t0);
+    const bool in = row < p.rows;
+    const int32_t query = in ? (int32_t)(row / group) : 0;
+    const int64_t token = p.qb + query, head = hk * group + (in ? row - (int64_t)query * group : 0);
+    const int32_t seen = in ? seen_by(a, p, query) : 0;
+    V q[D / 16];
 #pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const uint32_t i = d * 32 + e * 2 + hi * 4;
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (i + x < a.d) out[i + x] = o[d][e + x];
-            }
-        return;
+    for (int i = 0; i < D / 16; i++) {
+        q[i] = raw8((const T *)a.q + token * a.sq + head * a.sqh, i * 16 + hi * 8, a.d, in, (const T *)pl.zeros);
+        if (pl.negate) q[i] = -q[i];
     }
-    const float scale = 1.0f / total;
-    T *out = (T *)a.o + token * a.so + head * a.soh;
+    const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
+    const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
+    const uint32_t lds0 = lds_addr(lds);
+    auto load = [&](int32_t t) {
+        const uint32_t to = lds0 + (uint32_t)(t - t0) % ST * 2 * TILE;
+        const char *kb = kp + (uint64_t)t * KT * a.sk * 2, *vb = vp + (uint64_t)t * KT * a.sv * 2;
+        const uint32_t last = p.lk - 1 - t * KT;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const uint32_t idx = i * 64 + lane, r = idx / CH, from = min(r, last);
+            const uint32_t kc = ((idx % CH) ^ key_swizzle<D>(r)) * 8, vc = ((idx % CH) ^ value_swizzle<D>(r)) * 8;
+            if (kc < a.d)
+                lds_load16(kb, (from * (uint32_t)a.sk + kc) * 2, __builtin_amdgcn_readfirstlane(to + i * 1024));
+            if (vc < a.d)
+                lds_load16(vb, (from * (uint32_t)a.sv + vc) * 2, __builtin_amdgcn_readfirstlane(to + TILE + i * 1024));
+        }
+    };
+    v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const uint32_t i = d * 32 + e * 2 + hi * 4;
-            typedef T V4 __attribute__((ext_vector_type(4)));
-            typedef V4 V4U __attribute__((aligned(sizeof(T))));
-            V4 f;
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float top = -INFINITY, sum = 0;
+    bool not_finite = false;
+    const uint32_t vrow = hi * 4 + ((lane & 15) >> 2);
+    const uint32_t kat = lo * D * 2, vat = TILE + vrow * D * 2 + (lane & 1) * 8;
+    if (a.d < D) {  // what lies past d
+        for (uint32_t i = lane; i < ST * 2 * TILE / 16; i += 64) *(v4i *)(lds + i * 16) = v4i{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
 #pragma unroll
-            for (int x = 0; x < 4; x++) f[x] = (T)(seen > 0 ? o[d][e + x] * scale : 0.0f);
-            if (i + 4 <= a.d) {
-                *(V4U *)(out + i) = f;
-            } else {
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (i + x < a.d) out[i + x] = f[x];
-            }
+    for (int i = 0; i < ST - 1; i++)
+        if (t0 + i < t1) load(t0 + i);
+    for (int32_t t = t0; t < t1; t++) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the tile that the load replaces
+        if (t + ST - 1 < t1) {
+            load(t + ST - 1);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 1) * 2 * NL));
+        } else {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         }
+        asm volatile("" ::: "memory");
+        const unsigned char *buf = lds + (uint32_t)(t - t0) % ST * 2 * TILE;
+        if ((t + 1) * KT > all) {
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                not_finite |= any_not_finite(*(const v4i *)(buf + TILE + (i * 64 + lane) * 16), EXPONENT<T>);
+        }
+        v16f s;
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.0f;
+        V f[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) f[i] = *(const V *)(buf + kat + (((i * 2 + hi) ^ key_swizzle<D>(lo)) << 4));
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) s = mfma32(f[i], q[i], s);
+        if ((t + 1) * KT > all) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = t * KT + e / 4 * 8 + (int)hi * 4 + e % 4 < seen ? s[e] : -INFINITY;
+        }
+        float best = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; e++) best = fmaxf(best, s[e]);
+        best = halves_max(best) * pl.c;
+        if (__any(best > top + 8.0f)) {
+            const float now = fmaxf(top, best);
+            const float keep = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= keep;
+        }
+        const float m = top == -INFINITY ? 0.0f : top;
+        V w[2];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[e], pl.c, -m));
+            sum += x;
+            w[e / 8][e % 8] = (T)x;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                union {
+                    s16x4 half[2];
+                    V v;
+                } u;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint32_t c = (d * 4 + ((lane & 16) >> 3 | (lane & 2) >> 1)) ^ value_swizzle<D>(vrow);
+                    u.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4 *)(buf + vat + (c << 4) + (k * 16 + x * 8) * D * 2));
+                }
+                o[d] = mfma32(u.v, w[k], o[d]);
+            }
+    }
+    if (__any(not_finite)) {
+        float *own = (float *)lds;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int64_t i = p.row0; i < wend; i++)
+            row_alone<T>(a, pl, p, group, hk, i, t0 * KT, t1 * KT, split, own, own + 256);
+        return;
+    }
+    store_rows<T, D>(a, pl, o, top, sum, in, seen, token, head, split, t0 < t1);
 }
 
-// Joins the parts of a row, a wave each, in their order.
+// Joins the parts of a row, a workgroup each: a wave takes every fourth part.
+constexpr uint32_t MAX_SPLITS = 128;
 template <class T>
 __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, AttentionPlan pl, uint64_t first) {
-    const uint32_t group = a.hq / a.hk, lane = threadIdx.x & 63;
+    __shared__ float part[4][256];
+    const uint32_t group = a.hq / a.hk, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
-    if (!place_of(a, group, 4, first + blockIdx.x, p)) return;
-    const int64_t row = p.row0 + (threadIdx.x >> 6);
-    if (row >= p.rows) return;
-    const int32_t query = (int32_t)(row / group);
-    const int64_t token = p.qb + query, h = blockIdx.y * group + row % group;
+    if (!place_of(a, group, 1, first + blockIdx.x, p)) return;
+    const int32_t query = (int32_t)(p.row0 / group);
+    const int64_t token = p.qb + query, h = blockIdx.y * group + p.row0 % group;
     const uint64_t at = (uint64_t)token * a.hq + h, step = (uint64_t)a.tq * a.hq;
-    float top = -INFINITY;
-    for (uint32_t s = lane; s < pl.splits; s += 64) top = fmaxf(top, pl.part_ml[at + s * step].x);
-    top = wave_max(top);
-    float sum = 0, acc[4] = {};
-    for (uint32_t s = 0; s < pl.splits; s++) {
-        const float2 ml = pl.part_ml[at + s * step];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // a part with no key
-        const float keep = ml.x == top ? 1.0f : exp2f(ml.x - top);
-        sum = fmaf(ml.y, keep, sum);
-        const float *o = pl.part_o + (at + s * step) * a.d;
+    // lane s holds part s (and 64 + s)
+    constexpr int MANY = MAX_SPLITS / 64;
+    float2 ml[MANY];
+    float top = -INFINITY, sum = 0, acc[4] = {};
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-            if (c * 64 + lane < a.d) acc[c] = fmaf(o[c * 64 + lane], keep, acc[c]);
+    for (int i = 0; i < MANY; i++) {
+        const uint32_t s = i * 64 + lane;
+        ml[i] = s < pl.splits ? pl.part_ml[at + s * step] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[i].x);
     }
-    T *o = (T *)a.o + token * a.so + h * a.soh;
+    top = wave_max(top);
 #pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (c * 64 + lane < a.d) o[c * 64 + lane] = (T)(seen_by(a, p, query) > 0 ? acc[c] / sum : 0.0f);
+    for (int i = 0; i < MANY; i++) {
+        // a part with no key weighs nothing, and what its place holds is not used
+        const float keep = ml[i].x == top ? 1.0f : exp2f(ml[i].x - top);
+        ml[i].x = ml[i].x == -INFINITY && ml[i].y == 0.0f ? 0.0f : keep;
+        sum += ml[i].x * ml[i].y;
+    }
+    sum = wave_sum(sum);
+    for (uint32_t s0 = wave; s0 < pl.splits; s0 += 32) {  // eight parts' loads in flight
+        float x[8][4], keep[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t s = min(s0 + i * 4, pl.splits - 1);
+            keep[i] = __shfl(s < 64 ? ml[0].x : ml[1].x, s & 63);
+            keep[i] = s0 + i * 4 < pl.splits ? keep[i] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c * 64 < a.d) x[i][c] = pl.part_o[(at + s * step) * a.d + min(c * 64 + lane, a.d - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c * 64 < a.d) acc[c] += keep[i] == 0.0f ? 0.0f : x[i][c] * keep[i];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) part[wave][c * 64 + lane] = acc[c];
+    __syncthreads();
+    const uint32_t i = threadIdx.x;
+    if (i >= a.d) return;
+    const float o = part[0][i] + part[1][i] + part[2][i] + part[3][i];
+    ((T *)a.o)[token * a.so + h * a.soh + i] = (T)(seen_by(a, p, query) > 0 ? o / sum : 0.0f);
 }
+
+// Waves that are wanted: as many as the card holds at D = 128 (four a CU, one
+// round of 16 x 8192..16384 keys 51 us, two 56).
+constexpr uint64_t FEW_WAVES = 1024;
 
 // Keys of a tile: what two of keys and two of values leave of LDS and what a
 // wave's scores leave of its registers.  With turns between products and softmax
 // 128 keys a phase beat 64 by 3 to 5% (D = 128).
 constexpr uint32_t tile_keys(uint32_t d, uint32_t groups = 1) { return d > 128 ? 32 : groups == 2 && d >= 96 ? 128 : 64; }
 
-// Parts of the keys: where tiles of rows alone leave most of the card idle, and
-// no more than tiles of keys.
-uint32_t splits_of(const AttentionArgs &a) {
-    const uint64_t tiles = (a.tq * (a.hq / a.hk) / 128 + a.batch) * a.hk;
+// Rows of whole chunks at 16-byte addresses, near enough for 32-bit offsets.
+bool direct(const AttentionArgs &a) {
+    return a.d % 8 == 0 && std::max(a.sk, a.sv) < (1u << 24) && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 &&
+           (a.sk | a.skh | a.sv | a.svh) % 8 == 0;
+}
+// Whether a sequence's rows fit 32, as far as the caller says, or on average.
+bool few_rows(const AttentionArgs &a) {
+    const uint64_t queries = a.max_q ? a.max_q : (a.tq + a.batch - 1) / a.batch;
+    return queries * (a.hq / a.hk) <= 32 && a.d <= 128 && direct(a);
+}
+
+// Parts of the keys, where tiles of rows alone leave most of the card idle:
+// chunks of one length over all sequences, so that each part is as much work,
+// as long as `wanted` workgroups or waves need for all of them.
+uint32_t splits_of(const AttentionArgs &a, uint32_t *chunk) {
+    const bool few = few_rows(a);
+    const uint64_t rows = a.tq * (a.hq / a.hk) / (few ? 32 : 128) + a.batch, wanted = few ? FEW_WAVES : 512;
     const uint64_t keys = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
-    const uint64_t most = (keys + 4 * tile_keys(a.d) - 1) / (4 * tile_keys(a.d));
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({512 / tiles, most, 256}));
+    *chunk = 0;
+    if (wanted / (rows * a.hk) < (few ? 4 : 2)) return 1;  // (few: joining costs what it saves)
+    auto up = [](uint64_t x) { return (x + 127) / 128 * 128; };  // whole tiles, and not less than one of any kernel
+    uint64_t c = up(a.tk * (rows / a.batch) * a.hk / wanted);
+    c = std::max<uint64_t>({c, few ? 128u : 256u, up((keys + MAX_SPLITS - 1) / MAX_SPLITS)});
+    *chunk = (uint32_t)std::min<uint64_t>(c, 1u << 30);
+    return (uint32_t)std::max<uint64_t>(1, (keys + c - 1) / c);
 }
 
 template <class T, int D, int GROUPS, bool DIRECT>
@@ -555,11 +763,15 @@ hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipS
     // Turns pay where the products are as long as the softmax (D >= 96) and the
     // larger tiles of rows still fill the card: 16384 x 8 x 128 966 us against
     // 1028, D = 96 393 against 434, but D = 64 1250 against 1158.
-    if (DIRECT && D >= 96 && a.tq * (a.hq / a.hk) / 256 * a.hk >= 256)
+    if (DIRECT && D <= 128 && few_rows(a)) {
+        const uint64_t units = (a.tq * (a.hq / a.hk) / 32 + a.batch) * a.hk * pl.splits;
+        for (uint64_t f = 0; f < units; f += 4u << 23)
+            attention_few<T, D <= 128 ? D : 128><<<(uint32_t)std::min<uint64_t>((units - f + 3) / 4, 1u << 23), 256, 0, s>>>(a, pl, f, units);
+    } else if (DIRECT && D >= 96 && a.tq * (a.hq / a.hk) / 256 * a.hk >= 256)
         launch_tiles<T, D, DIRECT && D >= 96 ? 2 : 1, DIRECT>(a, pl, s);
     else launch_tiles<T, D, 1, DIRECT>(a, pl, s);
     if (pl.splits > 1) {
-        const uint64_t rows = a.tq * (a.hq / a.hk) / 4 + a.batch;
+        const uint64_t rows = a.tq * (a.hq / a.hk) + a.batch;
         for (uint64_t f = 0; f < rows; f += 1u << 23)
             attention_join<T><<<dim3((uint32_t)std::min<uint64_t>(rows - f, 1u << 23), a.hk), 256, 0, s>>>(a, pl, f);
     }
@@ -568,8 +780,7 @@ hipError_t attention_sized(const AttentionArgs &a, const AttentionPlan &pl, hipS
 
 template <class T>
 hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    const bool direct = a.d % 8 == 0 && std::max(a.sk, a.sv) < (1u << 24) && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && (a.sk | a.skh | a.sv | a.svh) % 8 == 0;
-    if (!direct) {
+    if (!direct(a)) {
         if (a.d <= 64) return attention_sized<T, 64, false>(a, pl, s);
         if (a.d <= 128) return attention_sized<T, 128, false>(a, pl, s);
         return attention_sized<T, 256, false>(a, pl, s);
@@ -584,7 +795,8 @@ hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStre
 }  // namespace
 
 size_t attention_workspace(const AttentionArgs &a) {
-    const uint32_t splits = splits_of(a);
+    uint32_t chunk;
+    const uint32_t splits = splits_of(a, &chunk);
     return splits > 1 ? (size_t)splits * a.tq * a.hq * (a.d + 2) * 4 : 0;
 }
 
@@ -592,7 +804,7 @@ hipError_t launch_attention(const AttentionArgs &a, void *ws, hipStream_t s) {
     AttentionPlan pl{};
     pl.c = std::fabs(a.scale) * 1.44269504f;
     pl.negate = a.scale < 0;
-    pl.splits = splits_of(a);
+    pl.splits = splits_of(a, &pl.chunk);
     pl.part_ml = (float2 *)ws;
     pl.part_o = (float *)ws + (size_t)pl.splits * a.tq * a.hq * 2;
     pl.zeros = a.zeros;
