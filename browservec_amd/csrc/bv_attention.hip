@@ -47,7 +47,7 @@ struct AttentionPlan {
 struct Place {
     int64_t qb, kb;      // first query and key of the sequence
     int32_t lq, lk;      // its lengths
-    int64_t rows, row0;  // its rows, the tile's first
+    int32_t rows, row0;  // its rows, the tile's first (all rows are fewer than 2^31)
 };
 __device__ __forceinline__ bool place_of(const AttentionArgs &a, uint32_t group, uint32_t tile, uint64_t slot, Place &p) {
     const uint32_t s = __builtin_amdgcn_readfirstlane(slot_sequence(a.cu_q, a.batch, a.tq, group, tile, slot));
@@ -55,10 +55,11 @@ __device__ __forceinline__ bool place_of(const AttentionArgs &a, uint32_t group,
     p.kb = clip_cu(a.cu_k, s, a.tk);
     p.lq = (int32_t)max((int64_t)0, clip_cu(a.cu_q, s + 1, a.tq) - p.qb);
     p.lk = (int32_t)max((int64_t)0, clip_cu(a.cu_k, s + 1, a.tk) - p.kb);
-    const int64_t nth = (int64_t)slot - p.qb * group / tile - s;
-    p.rows = (int64_t)p.lq * group;
-    p.row0 = nth * tile;
-    return nth >= 0 && p.row0 < p.rows;
+    const int64_t nth = (int64_t)slot - (uint32_t)p.qb * group / tile - s;
+    p.rows = p.lq * (int32_t)group;
+    if (nth < 0 || nth * tile >= p.rows) return false;
+    p.row0 = (int32_t)nth * (int32_t)tile;
+    return true;
 }
 // How many of the sequence's keys a query sees: the first ones.
 __device__ __forceinline__ int32_t seen_by(const AttentionArgs &a, const Place &p, int32_t query) {
@@ -102,28 +103,27 @@ __device__ __forceinline__ typename Vec8<T>::type raw8(const T *row, uint32_t at
     return v;
 }
 
-__device__ __forceinline__ bool any_not_finite(v4i v, uint32_t exponent) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t x = (uint32_t)v[i];
-        bad |= (x & exponent) == exponent || (x >> 16 & exponent) == exponent;
-    }
-    return bad;
-}
+// Whether one of eight elements is infinite or NaN: an exponent of ones carries
+// into the sign's place.
 template <class T>
-constexpr uint32_t EXPONENT = sizeof(T) && __is_same(T, f16) ? 0x7c00 : 0x7f80;
+__device__ __forceinline__ bool any_not_finite(v4i v) {
+    constexpr uint32_t EXPONENT = __is_same(T, f16) ? 0x7c007c00u : 0x7f807f80u, ONE = __is_same(T, f16) ? 0x04000400u : 0x00800080u;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) bad |= ((uint32_t)v[i] & EXPONENT) + ONE;
+    return bad & 0x80008000u;
+}
 
 // One row by one wave, reading only keys that it sees: for the rows of tiles
 // in which a value that some rows see and others do not is not finite (it
 // would reach those as 0 * inf in a matrix product).
 template <class T>
 __device__ __forceinline__ void row_alone(const AttentionArgs &a, const AttentionPlan &pl, const Place &p, uint32_t group,
-                                       uint32_t hk, int64_t row, int32_t j0, int32_t j1, uint32_t split, float *qs,
+                                       uint32_t hk, int32_t row, int32_t j0, int32_t j1, uint32_t split, float *qs,
                                        float *ps) {
     const uint32_t lane = threadIdx.x & 63;
-    const int32_t query = (int32_t)(row / group);
-    const int64_t token = p.qb + query, h = hk * group + row % group;
+    const int32_t query = (uint32_t)row / group;
+    const int64_t token = p.qb + query, h = hk * group + (uint32_t)row % group;
     const T *q = (const T *)a.q + token * a.sq + h * a.sqh;
     for (uint32_t i = lane; i < a.d; i += 64) qs[i] = (float)q[i] * (pl.negate ? -pl.c : pl.c);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -244,22 +244,22 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lo = lane & 31, hi = lane >> 5;
 
-    const int64_t row_end = min(p.rows, p.row0 + ROWS);
-    const int32_t seen_first = seen_by(a, p, (int32_t)(p.row0 / group));
-    const int32_t seen_last = seen_by(a, p, (int32_t)((row_end - 1) / group));
+    const int32_t row_end = min(p.rows, p.row0 + (int32_t)ROWS);
+    const int32_t seen_first = seen_by(a, p, (uint32_t)p.row0 / group);
+    const int32_t seen_last = seen_by(a, p, (uint32_t)(row_end - 1) / group);
     int32_t t0;
     const int32_t t1 = part_of<KT>(pl, split, seen_last, t0);
 
     // this wave's rows, and the tiles that some of them see
-    const int64_t wrow = p.row0 + wave * 32, wend = min(p.rows, wrow + 32);
-    const int32_t wave_all = wrow < p.rows ? seen_by(a, p, (int32_t)(wrow / group)) : 0;
-    const int32_t wave_any = wrow < p.rows ? seen_by(a, p, (int32_t)((wend - 1) / group)) : 0;
+    const int32_t wrow = p.row0 + wave * 32, wend = min(p.rows, wrow + 32);
+    const int32_t wave_all = wrow < p.rows ? seen_by(a, p, (uint32_t)wrow / group) : 0;
+    const int32_t wave_any = wrow < p.rows ? seen_by(a, p, (uint32_t)(wend - 1) / group) : 0;
     const int32_t tw = min(t1, (wave_any + KT - 1) / KT);
     const T *zeros = (const T *)pl.zeros;
-    const int64_t row = wrow + lo;
+    const int32_t row = wrow + lo;
     const bool in = row < p.rows;
-    const int32_t query = in ? (int32_t)(row / group) : 0;
-    const int64_t token = p.qb + query, head = hk * group + (in ? row - (int64_t)query * group : 0);
+    const int32_t query = in ? (uint32_t)row / group : 0;
+    const int64_t token = p.qb + query, head = hk * group + (in ? row - query * (int32_t)group : 0);
     const int32_t seen = in ? seen_by(a, p, query) : 0;
     V q[D / 16];
 #pragma unroll
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
 #pragma unroll
             for (int i = 0; i < NL; i++)
                 if (CHUNKS % THREADS == 0 || i * THREADS + wave * 64 < CHUNKS)
-                    not_finite |= any_not_finite(*(const v4i *)(lds + at + TILE + (i * THREADS + tid) * 16), EXPONENT<T>);
+                    not_finite |= any_not_finite<T>(*(const v4i *)(lds + at + TILE + (i * THREADS + tid) * 16));
         }
         if (t >= tw) return;
         V v[2][VB];
@@ -413,13 +413,11 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     auto softmax = [&](int32_t t) {
         if (t >= tw) return;
         if ((t + 1) * KT > wave_all) {
+            const int32_t left = seen - t * KT - (int)hi * 4;  // keys that the row sees, from this lane's first
 #pragma unroll
             for (int k = 0; k < KB; k++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int32_t j = t * KT + k * 32 + e / 4 * 8 + (int)hi * 4 + e % 4;
-                    s[k][e] = j < seen ? s[k][e] : -INFINITY;
-                }
+                for (int e = 0; e < 16; e++) s[k][e] = k * 32 + e / 4 * 8 + e % 4 < left ? s[k][e] : -INFINITY;
         }
         float best = -INFINITY;
 #pragma unroll
@@ -507,7 +505,7 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
 
     if (__syncthreads_or(not_finite)) {
         float *own = (float *)lds + wave * 320;
-        for (int64_t i = wrow; i < wend; i++)
+        for (int32_t i = wrow; i < wend; i++)
             row_alone<T>(a, pl, p, group, hk, i, t0 * KT, t1 * KT, split, own, own + 256);
         return;
     }
@@ -533,13 +531,13 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
     const uint32_t group = a.hq / a.hk, hk = (uint32_t)(unit % a.hk), split = (uint32_t)(unit / a.hk % pl.splits);
     Place p;
     if (!place_of(a, group, 32, unit / a.hk / pl.splits, p)) return;
-    const int64_t row = p.row0 + lo, wend = min(p.rows, p.row0 + 32);
-    const int32_t all = seen_by(a, p, (int32_t)(p.row0 / group)), any = seen_by(a, p, (int32_t)((wend - 1) / group));
+    const int32_t row = p.row0 + lo, wend = min(p.rows, p.row0 + 32);
+    const int32_t all = seen_by(a, p, (uint32_t)p.row0 / group), any = seen_by(a, p, (uint32_t)(wend - 1) / group);
     int32_t t0;
     const int32_t t1 = part_of<KT>(pl, split, any, t0);
     const bool in = row < p.rows;
-    const int32_t query = in ? (int32_t)(row / group) : 0;
-    const int64_t token = p.qb + query, head = hk * group + (in ? row - (int64_t)query * group : 0);
+    const int32_t query = in ? (uint32_t)row / group : 0;
+    const int64_t token = p.qb + query, head = hk * group + (in ? row - query * (int32_t)group : 0);
     const int32_t seen = in ? seen_by(a, p, query) : 0;
     V q[D / 16];
 #pragma unroll
@@ -593,7 +591,7 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
         if ((t + 1) * KT > all) {
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                not_finite |= any_not_finite(*(const v4i *)(buf + TILE + (i * 64 + lane) * 16), EXPONENT<T>);
+                not_finite |= any_not_finite<T>(*(const v4i *)(buf + TILE + (i * 64 + lane) * 16));
         }
         v16f s;
 #pragma unroll
@@ -604,8 +602,9 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
 #pragma unroll
         for (int i = 0; i < D / 16; i++) s = mfma32(f[i], q[i], s);
         if ((t + 1) * KT > all) {
+            const int32_t left = seen - t * KT - (int)hi * 4;
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = t * KT + e / 4 * 8 + (int)hi * 4 + e % 4 < seen ? s[e] : -INFINITY;
+            for (int e = 0; e < 16; e++) s[e] = e / 4 * 8 + e % 4 < left ? s[e] : -INFINITY;
         }
         float best = -INFINITY;
 #pragma unroll
@@ -649,7 +648,7 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
     if (__any(not_finite)) {
         float *own = (float *)lds;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int64_t i = p.row0; i < wend; i++)
+        for (int32_t i = p.row0; i < wend; i++)
             row_alone<T>(a, pl, p, group, hk, i, t0 * KT, t1 * KT, split, own, own + 256);
         return;
     }
@@ -664,8 +663,8 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a, Attention
     const uint32_t group = a.hq / a.hk, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Place p;
     if (!place_of(a, group, 1, first + blockIdx.x, p)) return;
-    const int32_t query = (int32_t)(p.row0 / group);
-    const int64_t token = p.qb + query, h = blockIdx.y * group + p.row0 % group;
+    const int32_t query = (uint32_t)p.row0 / group;
+    const int64_t token = p.qb + query, h = blockIdx.y * group + (uint32_t)p.row0 % group;
     const uint64_t at = (uint64_t)token * a.hq + h, step = (uint64_t)a.tq * a.hq;
     // lane s holds part s (and 64 + s)
     constexpr int MANY = MAX_SPLITS / 64;

@@ -123,7 +123,8 @@ __device__ __forceinline__ uint32_t slot_sequence(const int32_t *cu, uint32_t ba
     while (n > 1) {
         const uint32_t step = (n + 63) / 64;
         const uint32_t at = lane * step;
-        const bool past = at >= n || (uint64_t)(clip_cu(cu, lo + at, tokens) * group) / tile + lo + at > slot;
+        // tokens * group fits 32 bits
+        const bool past = at >= n || (uint64_t)((uint32_t)clip_cu(cu, lo + at, tokens) * group / tile) + lo + at > slot;
         const uint64_t not_past = __ballot(!past);
         // ascending offsets: the lanes not past are the first ones
         const uint32_t last = not_past ? 63 - __builtin_clzll(not_past) : 0;
