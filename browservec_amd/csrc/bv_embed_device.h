@@ -20,16 +20,19 @@ struct Vec8 {
     typedef type unaligned __attribute__((aligned(sizeof(T))));
 };
 
-template <class T>
+// ONCE: read once in all, not kept in the caches before other data
+template <bool ONCE = false, class T>
 __device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
-    const typename Vec8<T>::type v = *(const typename Vec8<T>::unaligned *)p;
+    typename Vec8<T>::type v;
+    if (ONCE) v = __builtin_nontemporal_load((const typename Vec8<T>::unaligned *)p);
+    else v = *(const typename Vec8<T>::unaligned *)p;
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = (float)v[i];
 }
 // Elements at..at+7 of a row of n, zeros past its end, without a branch per
 // lane: the load stays inside the row (ends with it) and its elements move down
 // by what it was too early.  tail: whether n is no multiple of 8.
-template <class T>
+template <bool ONCE = false, class T>
 __device__ __forceinline__ void load8(const T *row, uint32_t at, uint32_t n, bool tail, float (&f)[8]) {
     if (tail && n < 8) {
 #pragma unroll
@@ -40,7 +43,7 @@ __device__ __forceinline__ void load8(const T *row, uint32_t at, uint32_t n, boo
         return;
     }
     const uint32_t from = min(at, n - 8), early = at - from;
-    load8(row + from, f);
+    load8<ONCE>(row + from, f);
     if (tail) {
 #pragma unroll
         for (int step = 4; step; step /= 2)

@@ -131,11 +131,11 @@ __device__ __forceinline__ void load8_of(int type, const void *p, uint32_t at, u
 
 // What the norm does to each row: (f - mean) * r.
 template <int WAVES, int CH, int R>
-__device__ __forceinline__ void norm_stats(const NormArgs &a, uint32_t i, float *lds, const float (&f)[R][CH][8],
-                                           float (&mean)[R], float (&r)[R]) {
+__device__ __forceinline__ void norm_stats(const NormArgs &a, const int norm, uint32_t i, float *lds,
+                                           const float (&f)[R][CH][8], float (&mean)[R], float (&r)[R]) {
 #pragma unroll
     for (int k = 0; k < R; k++) mean[k] = 0.0f, r[k] = 1.0f;
-    if (a.norm == 1) {
+    if (norm == 1) {
         float sum[R] = {};
 #pragma unroll
         for (int k = 0; k < R; k++)
@@ -146,7 +146,7 @@ __device__ __forceinline__ void norm_stats(const NormArgs &a, uint32_t i, float 
 #pragma unroll
         for (int k = 0; k < R; k++) mean[k] = row_sum<WAVES>(sum[k], lds) / (float)a.dim;
     }
-    if (a.norm) {  // the squares about the mean, after it: no cancellation
+    if (norm) {  // the squares about the mean, after it: no cancellation
         float sq[R] = {};
 #pragma unroll
         for (int k = 0; k < R; k++)
@@ -154,7 +154,8 @@ __device__ __forceinline__ void norm_stats(const NormArgs &a, uint32_t i, float 
             for (int j = 0; j < CH; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float d = (j * 64 * WAVES + i) * 8 + e < a.dim ? f[k][j][e] - mean[k] : 0.0f;
+                    float d = f[k][j][e];
+                    if (norm == 1) d = (j * 64 * WAVES + i) * 8 + e < a.dim ? d - mean[k] : 0.0f;
                     sq[k] = fmaf(d, d, sq[k]);
                 }
 #pragma unroll
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256) void norm_rows(NormArgs a, uint64_t first) {
         }
     }
     float mean[R], r[R];
-    norm_stats<WAVES, CH, R>(a, i, lds, f, mean, r);
+    norm_stats<WAVES, CH, R>(a, a.norm, i, lds, f, mean, r);
 #pragma unroll
     for (int k = 0; k < R; k++)
 #pragma unroll
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(256) void norm_rows(NormArgs a, uint64_t first) {
 // Weights and biases are applied to the mean: they are the same for every row.
 constexpr uint32_t POOL_CHUNK = 64;
 
-template <class T, int WAVES, int CH, int R>
+template <class T, int WAVES, int CH, int NORM>
 __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
     constexpr int ROWS = 4 / WAVES;  // waves with rows of their own
     extern __shared__ float acc_lds[];
@@ -280,21 +281,17 @@ __global__ __launch_bounds__(256) void pool_chunk(NormArgs a, uint64_t first) {
     const uint32_t i = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, wave = WAVES == 1 ? threadIdx.x >> 6 : 0;
     const bool tail = a.dim % 8 != 0;
     float acc[1][CH][8] = {};
-    for (int64_t row = r0 + wave * R; row < r1; row += ROWS * R) {
-        float f[R][CH][8], mean[R], r[R];
+    for (int64_t row = r0 + wave; row < r1; row += ROWS) {
+        float f[1][CH][8], mean[1], r[1];
 #pragma unroll
-        for (int k = 0; k < R; k++)
+        for (int j = 0; j < CH; j++)
+            load8<true>((const T *)a.x + row * a.ldx, (j * 64 * WAVES + i) * 8, a.dim, tail, f[0][j]);
+        norm_stats<WAVES, CH, 1>(a, NORM, i, lds, f, mean, r);
 #pragma unroll
-            for (int j = 0; j < CH; j++)
-                load8((const T *)a.x + min(row + k, r1 - 1) * a.ldx, (j * 64 * WAVES + i) * 8, a.dim, tail, f[k][j]);
-        norm_stats<WAVES, CH, R>(a, i, lds, f, mean, r);
+        for (int j = 0; j < CH; j++)
 #pragma unroll
-        for (int k = 0; k < R; k++)
-            if (row + k < r1)
-#pragma unroll
-                for (int j = 0; j < CH; j++)
-#pragma unroll
-                    for (int x = 0; x < 8; x++) acc[0][j][x] += (f[k][j][x] - mean[k]) * r[k];
+            for (int x = 0; x < 8; x++)
+                acc[0][j][x] = fmaf(NORM == 1 ? f[0][j][x] - mean[0] : f[0][j][x], r[0], acc[0][j][x]);
     }
     if (ROWS > 1) {  // the waves' sums, by halves
         const uint32_t span = CH * 512;
@@ -367,7 +364,11 @@ hipError_t norm_of(const NormArgs &a, hipStream_t s) {
         const uint64_t chunks = pool_chunks(a.tokens, a.batch);
         const size_t lds = WAVES == 1 ? (size_t)2 * CH * 512 * 4 : 0;
         for (uint64_t c = 0; c < chunks; c += GRID_MOST)
-            pool_chunk<T, WAVES, CH, R><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c);
+            switch (a.norm) {
+            case 0: pool_chunk<T, WAVES, CH, 0><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c); break;
+            case 1: pool_chunk<T, WAVES, CH, 1><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c); break;
+            default: pool_chunk<T, WAVES, CH, 2><<<(uint32_t)std::min<uint64_t>(chunks - c, GRID_MOST), 256, lds, s>>>(a, c);
+            }
         if (a.tokens <= POOL_CHUNK) return hipGetLastError();  // every sequence fits one chunk
         for (uint64_t b = 0; b < a.batch; b += GRID_MOST) {
             const uint32_t n = (uint32_t)std::min<uint64_t>(a.batch - b, GRID_MOST);
