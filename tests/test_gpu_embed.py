@@ -98,6 +98,21 @@ def test_linear_many_tiles(ops, m, n, k):
     inside(ops.linear(x, w, bias=b, residual=r, activation="gelu"), *linear_want(x, w, b, r, "gelu", BF), "linear")
 
 
+@pytest.mark.parametrize("m,n,k", [(2100, 1500, 264), (10000, 1000, 136), (6000, 1500, 264), (8200, 4100, 520), (5000, 700, 1003)])
+def test_linear_large_tiles(ops, m, n, k):
+    """Every shape of tile, ragged at all three ends; 64-bit products on the GPU."""
+    say("linear large tiles", m, n, k)
+    x, w, b = rand((m, k), 1, HF).cuda(), rand((n, k), 2, HF, k ** -0.5).cuda(), rand((n,), 3, HF).cuda()
+    r = rand((m, n), 4, HF).cuda()
+    y = ops.linear(x, w, bias=b, residual=r, activation="silu")
+    xd, wd = x.double(), w.double()
+    z = (xd @ wd.t().contiguous() + b.double()).cpu()
+    mag = (xd.abs() @ wd.abs().t().contiguous() + b.double().abs()).cpu()
+    want = ACTS["silu"](z) + r.cpu().double()
+    bound = 1.13 * (k + 2) * 2.0 ** -23 * mag + 2.0 ** -20 * z.abs().clamp(min=1) + 2.0 ** -23 * want.abs()
+    inside(y, want, bound + U[HF] * (want.abs() + bound) + 2.0 ** -25, "large tiles")
+
+
 @pytest.mark.parametrize("m", [5, 300])
 @pytest.mark.parametrize("offset,extra", [(1, 3), (3, 8), (8, 16), (0, 1)])
 def test_linear_strides_and_alignment(ops, m, offset, extra):
@@ -301,6 +316,74 @@ def test_attention_ignores_what_it_does_not_see(ops, nq, nk):
         want, bound = attention_want(q[1:nq + 1], k2[3:nk + 3], v2[3:nk + 3], [0, nq], [0, nk], True)
         inside(o[1:1 + first], want[:first], bound[:first], f"unseen {value}")
         assert torch.all(o[0] == 9) and torch.all(o[nq + 1] == 9)  # queries of no sequence
+
+
+def attention_want_gpu(q, k, v, lens, causal):
+    """attention_want with its products on the GPU, for long sequences."""
+    u, out, bound = U[q.dtype], [], []
+    group, scale, a = q.shape[1] // k.shape[1], q.shape[2] ** -0.5, 0
+    for n in lens:
+        o, b = (torch.zeros(n, q.shape[1], q.shape[2], dtype=torch.float64) for _ in range(2))
+        for h in range(q.shape[1] if n else 0):
+            qq, kk, vv = (t[a:a + n, i].double() for t, i in ((q, h), (k, h // group), (v, h // group)))
+            s = scale * (qq @ kk.t().contiguous())
+            size = scale * (qq.abs() @ kk.abs().t().contiguous())
+            if causal:
+                unseen = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1)
+                s, size = s.masked_fill(unseen, float("-inf")), size.masked_fill(unseen, 0)
+            p = torch.exp(s - s.amax(1, keepdim=True))
+            total = p.sum(1, keepdim=True)
+            count = torch.arange(1, n + 1, device=q.device)[:, None] if causal else n
+            delta = (q.shape[2] + 2) * 2.0 ** -23 * size.amax(1, keepdim=True)
+            x = p @ vv / total
+            e = p @ vv.abs() / total * (u + 4 * delta + 2.0 ** -16 + 2 * count * 2.0 ** -24) + u * x.abs() * 1.01
+            if q.dtype == HF:
+                seen_v = torch.cumsum(vv.abs(), 0) if causal else vv.abs().sum(0, keepdim=True)
+                e += 2.0 ** -24 * (1 + seen_v / total)
+            o[:, h], b[:, h] = x.cpu(), e.cpu()
+        out.append(o)
+        bound.append(b)
+        a += n
+    return torch.cat(out), torch.cat(bound)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("hq,hk,d,dtype", [(16, 4, 128, BF), (8, 8, 80, HF), (12, 3, 96, BF), (16, 4, 256, HF), (24, 8, 64, BF)])
+def test_attention_long_packed(ops, hq, hk, d, dtype, causal):
+    """Enough rows that a call fills the card: the tiles that only then run."""
+    lens = [3000, 1, 0, 2100, 77, 6000 if hq == hk else 130]
+    say("attention long", lens, hq, hk, d, dtype, causal)
+    t = sum(lens)
+    q, k, v = rand((t, hq, d), 1, dtype, 1.5).cuda(), rand((t, hk, d), 2, dtype).cuda(), rand((t, hk, d), 3, dtype).cuda()
+    o = ops.attention(q, k, v, dev_cu(cu_of(lens)), causal=causal)
+    inside(o, *attention_want_gpu(q, k, v, lens, causal), "attention long")
+    if causal:  # a value near the end that is not finite: nothing before it changes, everything after does
+        v[2990, :, d // 2] = float("nan")
+        again = ops.attention(q, k, v, dev_cu(cu_of(lens)), causal=True)
+        same = torch.ones(t, dtype=torch.bool)
+        same[2990:3000] = False
+        # (rows done one by one round otherwise: within twice the bound of each other)
+        want, bound = attention_want_gpu(q[:2990], k[:2990], v[:2990], [2990], True)
+        inside(again[:2990], want, bound, "before the NaN")
+        assert torch.equal(again[3000:], o[3000:])
+        assert torch.isnan(again[2990:3000, :, d // 2]).all() and not torch.isnan(again[2990:3000, :, :d // 2]).any()
+
+
+def test_many_short_sequences(ops):
+    """Thousands of sequences of one token or none: attention gives the value, the mean is the row."""
+    say("many short sequences")
+    n, hq, hk, d = 9000, 4, 2, 64
+    lens = [1 if i % 7 else 0 for i in range(n)]
+    t, cu = sum(lens), dev_cu(cu_of(lens))
+    q, k, v = rand((t, hq, d), 1, BF).cuda(), rand((t, hk, d), 2, BF).cuda(), rand((t, hk, d), 3, BF).cuda()
+    for hint in (0, 1):
+        assert torch.equal(ops.attention(q, k, v, cu, max_q=hint, max_k=hint), v.repeat_interleave(2, 1))
+    x = rand((t, 40), 4, F32).cuda()
+    got = ops.pool(x, cu, unit=False)
+    live = torch.tensor(lens, dtype=torch.bool)
+    assert torch.equal(got.cpu()[live], x.cpu()) and torch.all(got.cpu()[~live] == 0)
+    for mode in ("first", "last"):
+        assert torch.equal(ops.pool(x, cu, mode=mode, unit=False), got)
 
 
 def test_attention_large_scores(ops):
