@@ -240,7 +240,8 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     // where 8 is a multiple of their number, an XCD reads those of one.
     const uint32_t group = a.hq / a.hk, nth = blockIdx.x / a.hk, hk = blockIdx.x - nth * a.hk, split = blockIdx.z;
     Place p;
-    if (!place_of(a, group, ROWS, first + gridDim.x / a.hk - 1 - nth, p)) return;
+    const uint32_t slots = gridDim.x / a.hk;
+    if (!place_of(a, group, ROWS, first + slots - 1 - spread(nth, slots, a.hk), p)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lo = lane & 31, hi = lane >> 5;
 

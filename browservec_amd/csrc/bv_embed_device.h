@@ -137,5 +137,18 @@ __device__ __forceinline__ uint32_t slot_sequence(const int32_t *cu, uint32_t ba
     return lo;
 }
 
+// Slots without a tile come at steps that the lengths give, every second one
+// where sequences fill a tile each, and workgroups go to XCDs, and there to
+// shader engines, in turn: taken in order, half of the card would idle.  So of
+// `each` workgroups a slot, i-th of n slots: an XCD takes two neighbouring ones,
+// in an order that changes from two to two.  Attention over 512 x 128 tokens, 8
+// heads of 64: 81 us, in order 133; pooling 1111 x 16 rows of 3904 66 and 103.
+__device__ __forceinline__ uint32_t spread(uint32_t i, uint32_t n, uint32_t each) {
+    const uint32_t lg = 3 - min(3, (int)__builtin_ctz(each));  // after 2^lg slots XCDs repeat
+    const uint32_t group = i >> (1 + lg), l = i & ((2 << lg) - 1);
+    if ((group + 1) << (1 + lg) > n) return i;
+    return (group << (1 + lg)) + 2 * (l & ((1 << lg) - 1)) + ((l >> lg) ^ (group * 0x9e3779b9u >> 31));
+}
+
 }  // namespace
 }  // namespace bvk
