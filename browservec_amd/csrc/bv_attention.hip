@@ -227,6 +227,12 @@ __device__ __forceinline__ void store_rows(const AttentionArgs &a, const Attenti
 //     GROUPS 1 that share a CU fall into step, both waves of a SIMD multiplying
 //     and then both computing weights: 2300 cycles a tile and wave at D = 128
 //     where the products take 1024.)
+// Bound by the matrix cores and the vector unit together: at D = 128 they overlap
+// but for the turns' ends and the clock that the products leave (9001 and 16001
+// tokens, 8 heads over 2, causal, f16: 863 us, 1020 TFLOP/s), at D = 64 the
+// exponentials and their bookkeeping take longer than the products (96 x 1..512
+// tokens, 12 heads over 4, causal: 46 us, where the start of a workgroup also
+// counts).  With turns, D = 128 spills 2 registers a lane and D = 256 23.
 template <class T, int D, int KT, int GROUPS, bool DIRECT>
 __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {
@@ -516,8 +522,10 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
 // Few rows a sequence (the next tokens over kept keys): what counts is to
 // stream keys and values.  Each wave works alone: 32 rows of one key head over
 // its part of the keys, 32 at a time through two tiles of its own in LDS, one on
-// its way; no barriers.  Neighbouring waves take the key heads side
-// by side in memory.
+// its way; no barriers.  Neighbouring waves take the key heads side by side in
+// memory.  Bound by the read of keys and values and the start of their chain:
+// 8 sequences of up to 32768 keys, 4 key heads of 64, one new token each: 25 us, and
+// 6 to join.
 template <class T, int D>
 __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, AttentionPlan pl, uint64_t first, uint64_t units) {
     typedef typename Vec8<T>::type V;
