@@ -520,6 +520,24 @@ def test_pool(ops, lens, dim, dtype, kind, mode):
         inside(got, want, bound, f"pool {mode} {kind} unit {unit}")
 
 
+@pytest.mark.parametrize("dim,dtype,kind", [(384, BF, "rms"), (1000, HF, None), (2500, BF, "layer"), (3901, F32, None), (5000, HF, "rms"), (9001, BF, "layer")])
+def test_pool_many_sequences(ops, dim, dtype, kind):
+    """More sequences than compute units, of none, one or several chunks."""
+    say("pool many", dim, dtype, kind)
+    lens = [(0, 1, 16, 17, 33, 5, 64, 2)[i % 8] for i in range(299)] + [140]
+    cu = cu_of(lens)
+    x = rand((cu[-1], dim), 1, dtype, 1.0, 0.3)
+    rows, err = norm_want(x, None, None, kind)
+    want, bound = torch.zeros(len(lens), dim, dtype=torch.float64), torch.zeros(len(lens), dim, dtype=torch.float64)
+    for s, (a, e) in enumerate(zip(cu, cu[1:])):
+        if e > a:  # a row's elements are added one by one at most
+            want[s] = rows[a:e].mean(0)
+            bound[s] = err[a:e].mean(0) + (e - a + 2) * 2.0 ** -24 * rows[a:e].abs().mean(0) + 1e-37
+    got = ops.pool(x.cuda(), dev_cu(cu), kind=kind, unit=False)
+    inside(got, want, bound, "pool many")
+    assert torch.equal(got, ops.pool(x.cuda(), dev_cu(cu), kind=kind, unit=False))
+
+
 def test_pool_zero_vector_and_far_rows(ops):
     say("pool zero vector")
     x = torch.zeros(5, 64, dtype=BF, device="cuda")
