@@ -120,30 +120,34 @@ hipError_t rotary_of(const RotaryArgs &a, hipStream_t s) {
 template <int WAVES>
 constexpr int BLOCK = WAVES <= 4 ? 256 : 64 * WAVES;
 
-// Sums over a row's threads, of R rows at once.  Waves exchange theirs through
-// two places in turn, with one barrier a sum: a place is written again after the
-// next sum's barrier, which every reader has reached by then.
+// Sums over a row's threads, of up to R rows at once.  Waves exchange theirs
+// through two places in turn, with one barrier a sum: a place is written again
+// after the next sum's barrier, which every reader has reached by then.  That
+// holds for sums of fewer rows too, since the places lie WAVES * R apart whatever
+// a sum's rows: all sums of a workgroup go through one of these.
 template <int WAVES, int R>
 struct RowSums {
-    static constexpr int FLOATS = 2 * WAVES * R;
+    static constexpr int PLACE = WAVES * R, FLOATS = 2 * PLACE;
     float *lds;
     int turn = 0;
-    __device__ __forceinline__ void operator()(float (&x)[R]) {
+    template <int K>
+    __device__ __forceinline__ void operator()(float (&x)[K]) {
+        static_assert(WAVES * K <= PLACE, "a sum stays within its place");
 #pragma unroll
-        for (int k = 0; k < R; k++) x[k] = wave_sum(x[k]);
+        for (int k = 0; k < K; k++) x[k] = wave_sum(x[k]);
         if (WAVES == 1) return;
-        float *p = lds + turn * WAVES * R;
+        float *p = lds + turn * PLACE;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
-            for (int k = 0; k < R; k++) p[(threadIdx.x >> 6) * R + k] = x[k];
+            for (int k = 0; k < K; k++) p[(threadIdx.x >> 6) * K + k] = x[k];
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < R; k++) x[k] = 0;
+        for (int k = 0; k < K; k++) x[k] = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; w++)
 #pragma unroll
-            for (int k = 0; k < R; k++) x[k] += p[w * R + k];
+            for (int k = 0; k < K; k++) x[k] += p[w * K + k];
     }
 };
 
@@ -210,8 +214,8 @@ __device__ __forceinline__ void weighted(const NormArgs &a, uint32_t i, float (&
 }
 
 // Rows y0 on, `rows` of them: y = f, unit: f times 1 / |f| (a zero row stays).
-template <class O, int WAVES, int CH, int R>
-__device__ __forceinline__ void store_rows(const NormArgs &a, O *y0, uint64_t rows, uint32_t i, RowSums<WAVES, R> &sums,
+template <class O, int WAVES, int CH, int R, int MOST>
+__device__ __forceinline__ void store_rows(const NormArgs &a, O *y0, uint64_t rows, uint32_t i, RowSums<WAVES, MOST> &sums,
                                            float (&f)[R][CH][8]) {
     if (a.unit) {
         float sq[R] = {};
@@ -375,8 +379,7 @@ __global__ __launch_bounds__(BLOCK<WAVES>) void pool_chunk(NormArgs a, uint64_t 
 #pragma unroll
         for (int x = 0; x < 8; x++) acc[0][j][x] *= inv;
     if (e > b) weighted<WAVES, CH, 1>(a, i, acc);
-    RowSums<WAVES, 1> one{lds, sums.turn};
-    store_rows<float, WAVES, CH, 1>(a, (float *)a.y + (uint64_t)s * a.ldy, 1, i, one, acc);
+    store_rows<float, WAVES, CH, 1>(a, (float *)a.y + (uint64_t)s * a.ldy, 1, i, sums, acc);
 }
 
 // A sequence a workgroup of JOIN waves, of which groups of WAVES take the parts
