@@ -200,8 +200,9 @@ class EmbedOps:
     def _turned(self, x, out):
         if out is None:
             return _heads(x), self._empty(x.shape, dtype=x.dtype, device=x.device)
-        if out.shape != x.shape or out.dtype != x.dtype or (out.shape[2] > 1 and out.stride(2) != 1):
-            _bad("rotary: an output differs from its input in shape or type, or its last dimension is not contiguous")
+        if out.shape != x.shape or out.dtype != x.dtype:
+            _bad("rotary: an output differs from its input in shape or type")
+        _out_heads(out, "rotary")
         return (x if out is x else _heads(x)), out
 
     def attention(self, q, k, v, cu_q, cu_k=None, max_q: int = 0, max_k: int = 0, causal: bool = True, scale: float | None = None,
@@ -227,8 +228,10 @@ class EmbedOps:
             _bad("attention: cu_q and cu_k differ in length, or max_q or max_k is negative")
         if out is None:
             out = self._empty(sq, dtype=dtype, device=q.device)
-        elif out.shape != sq or out.dtype != dtype or (sq[2] > 1 and out.stride(2) != 1):
-            _bad("attention: out differs from q in shape or type, or its last dimension is not contiguous")
+        elif out.shape != sq or out.dtype != dtype:
+            _bad("attention: out differs from q in shape or type")
+        else:
+            _out_heads(out, "attention")
         q, k, v = _heads(q), _heads(k), _heads(v)
         a.dtype, a.causal, a.batch = self._dtype(q, "attention"), bool(causal), cu_q.shape[0] - 1
         a.tokens_q, a.heads_q, a.head_dim = sq
@@ -316,7 +319,20 @@ def _out_stride(y, what: str) -> int:
     step, one = y.stride()
     if one != 1 and n > 1:
         _bad(f"{what}: out's last dimension is not contiguous")
+    if rows > 1 and step < n:  # an expanded tensor's 0 among them, which would mean packed
+        _bad(f"{what}: out's rows overlap")
     return step if rows > 1 else 0
+
+
+def _out_heads(out, what: str) -> None:
+    """Refuses what the library would take for packed heads (other strides that
+    make heads overlap it refuses itself)."""
+    tokens, heads, d = out.shape
+    st, sh, one = out.stride()
+    if one != 1 and d > 1:
+        _bad(f"{what}: out's last dimension is not contiguous")
+    if (st == 0 and tokens > 1) or (sh == 0 and heads > 1):
+        _bad(f"{what}: out's rows overlap")
 
 
 def _heads(t):

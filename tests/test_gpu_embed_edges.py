@@ -38,3 +38,36 @@ def test_pool_unit_of_wide_rms_rows(ops, dim, dtype):  # noqa: F811
     inside(got, want, bound, "unit of wide rows")
     for _ in range(5):
         assert torch.equal(ops.pool(x, c, kind="rms", weight=w), got)
+
+
+# ------------------------------------------------------------------ outputs --
+def test_outputs_that_overlap_themselves_are_refused(ops):  # noqa: F811
+    """An expanded output holds fewer elements than its shape says."""
+    from browservec_amd import _lib as L
+    from browservec_amd import rotary_table
+
+    say("outputs that overlap themselves")
+    x, w = rand((6, 16), 1, BF).cuda(), rand((16, 16), 2, BF).cuda()
+    q, cu, table = rand((6, 2, 8), 3, BF).cuda(), dev_cu([0, 6]), torch.from_numpy(rotary_table(6, 8)).cuda()
+    row, head = torch.zeros(1, 16, dtype=BF, device="cuda"), torch.zeros(1, 1, 8, dtype=BF, device="cuda")
+    one = torch.zeros(1, 16, dtype=F32, device="cuda")
+    for fn in (
+        lambda: ops.linear(x, w, out=row.expand(6, 16)),
+        lambda: ops.linear(x, w, residual=row.expand(6, 16), out=row.expand(6, 16)),
+        lambda: ops.linear(x.unflatten(0, (2, 3)), w, out=row.expand(2, 3, 16)),
+        lambda: ops.norm(x, out=row.expand(6, 16)),
+        lambda: ops.pool(x, dev_cu([0, 2, 6]), out=one.expand(2, 16)),
+        lambda: ops.attention(q, q, q, cu, out=head.expand(6, 2, 8)),
+        lambda: ops.attention(q[:1], q, q, dev_cu([0, 1]), cu, out=head.expand(1, 2, 8)),
+        lambda: ops.rotary(q, None, table, out_q=head.expand(6, 2, 8)),
+        lambda: ops.rotary(q, q.clone(), table, out_k=torch.zeros(6, 1, 8, dtype=BF, device="cuda").expand(6, 2, 8)),
+    ):
+        with pytest.raises(L.BVError) as e:
+            fn()
+        assert e.value.code == L.BV_E_INVALID
+    assert not row.any() and not head.any() and not one.any()
+    e = row.expand(6, 16)  # in place, of the input itself
+    with pytest.raises(L.BVError):
+        ops.norm(e, out=e)
+    # inputs may be expanded: they are copied
+    inside(ops.linear(x[:1].expand(6, 16), w), *linear_want(x[:1].expand(6, 16), w, None, None, "none", BF), "expanded input")
