@@ -370,6 +370,9 @@ extern "C" int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *ar
     if (a.head_dim > 256) return fail(BV_E_UNSUPPORTED, "attention: head_dim %u exceeds 256", a.head_dim);
     if (a.tokens_q > TOKENS_MOST || a.tokens_k > TOKENS_MOST || a.batch > TOKENS_MOST)
         return fail(BV_E_INVALID, "attention: tokens and batch are at most 2^31 - 1");
+    // tiles that hold a sequence's last rows and keys end past them, in 32 bits
+    if (a.tokens_k > TOKENS_MOST - 1024)
+        return fail(BV_E_UNSUPPORTED, "attention: %llu keys, at most 2^31 - 1025", (unsigned long long)a.tokens_k);
     if (a.tokens_q * (a.heads_q / a.heads_k) > TOKENS_MOST - 1024)
         return fail(BV_E_UNSUPPORTED, "attention: %llu queries of %u heads a key head, at most 2^31 - 1025 in all",
                     (unsigned long long)a.tokens_q, a.heads_q / a.heads_k);

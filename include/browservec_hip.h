@@ -461,7 +461,8 @@ int bv_embed_rotary_table(const bv_embed_rotary_scaling *scaling, uint32_t table
  * queries cu_q[s] to cu_q[s+1] of q [tokens_q][heads_q][head_dim] and the keys
  * cu_k[s] to cu_k[s+1] of k, v [tokens_k][heads_k][head_dim] (dtype BV_F16 or
  * BV_BF16; head_dim at most 256; heads_q a multiple of heads_k, query head h
- * reads key head h / (heads_q/heads_k)).  cu_q, cu_k: batch + 1 ascending
+ * reads key head h / (heads_q/heads_k); tokens_k and tokens_q heads_q/heads_k
+ * at most 2^31 - 1025).  cu_q, cu_k: batch + 1 ascending
  * int32, clipped to the tokens there are.  causal: a sequence's last query
  * sees its last key, each query before it one key less.  A query that sees no
  * key gives zeros.  Keys and values that a query does not see have no effect

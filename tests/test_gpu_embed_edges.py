@@ -71,3 +71,51 @@ def test_outputs_that_overlap_themselves_are_refused(ops):  # noqa: F811
         ops.norm(e, out=e)
     # inputs may be expanded: they are copied
     inside(ops.linear(x[:1].expand(6, 16), w), *linear_want(x[:1].expand(6, 16), w, None, None, "none", BF), "expanded input")
+
+
+# --------------------------------------------------------- attention, sizes --
+def attention_args(**kw):
+    """One query head over one key head of 8 elements, packed, pointers that the checks accept."""
+    from browservec_amd import _lib as L
+
+    buf = torch.zeros(4096, dtype=BF, device="cuda")
+    p = buf.data_ptr()
+    a = L.AttentionArgs(ctypes.sizeof(L.AttentionArgs), 2, 1, 1, 8, 1, 1)
+    a.tokens_q, a.tokens_k, a.q, a.k, a.v, a.o, a.cu_q, a.cu_k = 1, 1, p, p + 64, p + 128, p + 192, p + 256, p + 320
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a, buf
+
+
+@pytest.mark.parametrize("tokens_k", [2 ** 31 - 1024, 2 ** 31 - 128, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
+def test_attention_of_too_many_keys_is_refused(ops, tokens_k):  # noqa: F811
+    """A tile's end has to fit 32 bits as well."""
+    from browservec_amd import _lib as L
+
+    say("attention, too many keys", tokens_k)
+    a, buf = attention_args(tokens_k=tokens_k)
+    assert L.load().bv_embed_attention(ops.handle, ctypes.addressof(a)) in (L.BV_E_INVALID, L.BV_E_UNSUPPORTED)
+    assert b"attention" in L.load().bv_last_error()
+    ops.sync()
+
+
+@pytest.mark.parametrize("d", [1, 8])
+def test_attention_of_the_most_keys(ops, d):  # noqa: F811
+    """One sequence of as many keys as a call takes: the last one counts most,
+    and the rest not nothing."""
+    n = 2 ** 31 - 1025
+    say("attention, the most keys", d)
+    if torch.cuda.mem_get_info()[0] < 2 * n * d * 2 + 2 ** 32:
+        pytest.skip("not enough device memory free")
+    q = torch.ones(1, 1, d, dtype=BF, device="cuda")
+    k, v = torch.zeros(n, 1, d, dtype=BF, device="cuda"), torch.ones(n, 1, d, dtype=BF, device="cuda")
+    k[-1, 0, 0] = 22.0  # its weight against 2^31 others of 1: e^22 = 3.6e9
+    v[-1] = -1.0
+    o = ops.attention(q, k, v, dev_cu([0, 1]), dev_cu([0, n]), scale=1.0)
+    top = torch.exp(torch.tensor(22.0, dtype=torch.float64))
+    want = ((n - 1 - top) / (n - 1 + top)).expand(1, 1, d)
+    # weights are exact but for the last one's exponential, within 2^-17 of its
+    # value, and sums of 2^31 terms by 128 parts of 2^24, each exact in 32 bits up to 2^24
+    inside(o, want, U[BF] * want.abs() * 1.01 + 2 * 2.0 ** -16, "the most keys")
+    del q, k, v, o
+    torch.cuda.empty_cache()
