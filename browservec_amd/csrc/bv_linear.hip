@@ -356,14 +356,14 @@ __global__ __launch_bounds__(ROW_WAVES * 64) void linear_rows(LinearArgs a) {
         V wv, xv;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const T e = w[kc + i < left ? (int)(k + i) : -(int)kc];
+            const T e = w[kc + i < left ? (int64_t)(k + i) : -(int64_t)kc];
             wv[i] = kc + i < left ? e : (T)0.0f;
         }
 #pragma unroll
         for (int m = 0; m < MF; m++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const T e = x[m][kc + i < left ? (int)(k + i) : -(int)kc];
+                const T e = x[m][kc + i < left ? (int64_t)(k + i) : -(int64_t)kc];
                 xv[i] = kc + i < left ? e : (T)0.0f;
             }
             acc[m] = mfma16(wv, xv, acc[m]);

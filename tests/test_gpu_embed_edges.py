@@ -119,3 +119,19 @@ def test_attention_of_the_most_keys(ops, d):  # noqa: F811
     inside(o, want, U[BF] * want.abs() * 1.01 + 2 * 2.0 ** -16, "the most keys")
     del q, k, v, o
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------ linear, sizes --
+def test_linear_of_rows_past_32_bits(ops):  # noqa: F811
+    """The elements after the last whole step lie past 2^31 in their row."""
+    k = 2 ** 31 + 5
+    say("linear, rows of 2^31 + 5")
+    if torch.cuda.mem_get_info()[0] < 5 * 2 ** 32:
+        pytest.skip("not enough device memory free")
+    x, w = torch.zeros(1, k, dtype=BF, device="cuda"), torch.zeros(1, k, dtype=BF, device="cuda")
+    for at, a, b in ((0, 3, 5), (2 ** 31 - 1, 2, 7), (2 ** 31, 4, 11), (k - 1, 8, 13)):
+        x[0, at], w[0, at] = a, b
+    y = ops.linear(x, w, out_dtype=F32)
+    assert y.item() == 3 * 5 + 2 * 7 + 4 * 11 + 8 * 13  # exact in 32 bits
+    del x, w
+    torch.cuda.empty_cache()
