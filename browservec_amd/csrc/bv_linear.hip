@@ -418,10 +418,14 @@ __global__ __launch_bounds__(256) void pack_rows(const T *x, uint64_t ldx, uint3
 // Rows up to which w goes straight to the registers: 32 rows, 4096 x 4096: 15.8
 // us, by tiles 17.7; 64 rows 21.7 and 19.2.
 constexpr uint64_t FEW_ROWS = 32;
+// A tile's loads have 32-bit offsets: 256 rows of as many elements reach 2^31
+// bytes.  Rows further apart are packed, longer rows go 32 at a time.
+constexpr uint64_t FAR_ROWS = 1u << 22;
 
 bool aligned(const void *p, uint64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+bool by_rows(const LinearArgs &a) { return a.m <= FEW_ROWS || a.k >= FAR_ROWS; }
 bool packs(const LinearArgs &a, const void *p, uint64_t ld) {
-    return a.m > FEW_ROWS && a.k && (a.k % 8 || !aligned(p, ld) || ld >= (1u << 22));
+    return !by_rows(a) && a.k && (a.k % 8 || !aligned(p, ld) || ld >= FAR_ROWS);
 }
 uint64_t packed_bytes(uint64_t rows, uint32_t k) { return (rows * ((k + 7) / 8) * 16 + 255) & ~255ull; }
 
@@ -461,9 +465,17 @@ hipError_t rows_of(const LinearArgs &a, hipStream_t s) {
 
 template <class T, class O>
 hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
-    if (a.m <= FEW_ROWS) {
-        if (a.m <= 16) return rows_of<T, O, 1>(a, s);
-        return rows_of<T, O, 2>(a, s);
+    if (by_rows(a)) {
+        for (uint64_t m = 0; m < a.m; m += FEW_ROWS) {
+            LinearArgs b = a;
+            b.m = std::min(a.m - m, FEW_ROWS);
+            b.x = (const T *)a.x + m * a.ldx;
+            b.y = (O *)a.y + m * a.ldy;
+            if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
+            const hipError_t e = b.m <= 16 ? rows_of<T, O, 1>(b, s) : rows_of<T, O, 2>(b, s);
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
     }
     const bool px = packs(a, a.x, a.ldx), pw = packs(a, a.w, a.ldw);
     if (px) {

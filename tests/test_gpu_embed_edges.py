@@ -135,3 +135,22 @@ def test_linear_of_rows_past_32_bits(ops):  # noqa: F811
     assert y.item() == 3 * 5 + 2 * 7 + 4 * 11 + 8 * 13  # exact in 32 bits
     del x, w
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 3, 2 ** 26), (33, 17, 2 ** 22 + 3)])
+def test_linear_of_long_rows(ops, m, n, k):  # noqa: F811
+    """Tens of rows so long that some lie 2^32 bytes and more after the first,
+    as one tile would address them."""
+    say("linear, long rows", m, n, k)
+    if torch.cuda.mem_get_info()[0] < 2 * (m + n) * k + 2 ** 32:
+        pytest.skip("not enough device memory free")
+    x, w = torch.zeros(m, k, dtype=BF, device="cuda"), torch.zeros(n, k, dtype=BF, device="cuda")
+    a, b = torch.arange(1, m + 1).to(BF).cuda(), torch.arange(1, n + 1).to(BF).cuda()
+    for at in (0, 1000, k - 1):
+        x[:, at], w[:, at] = a, b
+    r = rand((m, n), 3, BF).round().cuda()
+    y = ops.linear(x, w, residual=r, out=torch.empty(m, n + 5, dtype=BF, device="cuda")[:, 2:n + 2])
+    want = 3 * a.double()[:, None] * b.double() + r.double()  # exact in 32 bits, rounded once
+    assert torch.equal(y, want.to(BF))
+    del x, w
+    torch.cuda.empty_cache()
