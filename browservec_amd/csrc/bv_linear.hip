@@ -439,19 +439,35 @@ hipError_t pack(const void *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *t
     return hipGetLastError();
 }
 
+// A launch holds fewer than 2^32 threads, of more it runs the low 32 bits: so
+// many workgroups of at most 1024 at a time.
+constexpr uint32_t GRID_MOST = 1u << 21;
+
+// The part of a call that makes rows m to m + rows and columns n to n + cols.
+template <class T, class O>
+LinearArgs part_of(const LinearArgs &a, uint64_t m, uint64_t rows, uint64_t n, uint64_t cols) {
+    LinearArgs b = a;
+    b.m = std::min(a.m - m, rows);
+    b.n = (uint32_t)std::min(a.n - n, cols);
+    b.x = (const T *)a.x + m * a.ldx;
+    b.w = (const T *)a.w + n * a.ldw;
+    b.y = (O *)a.y + m * a.ldy + n;
+    if (a.bias) b.bias = (const T *)a.bias + n;
+    if (a.residual) b.residual = (const O *)a.residual + m * a.ldr + n;
+    return b;
+}
+
 template <class T, class O, int BM, int BN, int WN, int BK, int ST, int KG = 1>
 hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
-    const uint32_t tn = (a.n + BN - 1) / BN;
-    // a launch holds fewer than 2^32 threads
-    const uint64_t most = std::max<uint64_t>(1, (1u << 22) / tn);
-    for (uint64_t m = 0; m < a.m; m += most * BM) {
-        LinearArgs b = a;
-        b.m = std::min(a.m - m, most * BM);
-        b.x = (const T *)a.x + m * a.ldx;
-        b.y = (O *)a.y + m * a.ldy;
-        if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
-        const uint32_t tm = (uint32_t)((b.m + BM - 1) / BM);
-        linear_tile<T, O, BM, BN, WN, BK, ST, KG><<<tm * tn, 128 * WN * KG, 0, s>>>(b, tm, tn);
+    static_assert(128 * WN * KG <= 1024, "GRID_MOST is for 1024 threads");
+    for (uint64_t n = 0; n < a.n; n += (uint64_t)GRID_MOST * BN) {
+        const uint32_t tn = (uint32_t)((std::min<uint64_t>(a.n - n, (uint64_t)GRID_MOST * BN) + BN - 1) / BN);
+        const uint64_t most = GRID_MOST / tn;
+        for (uint64_t m = 0; m < a.m; m += most * BM) {
+            const LinearArgs b = part_of<T, O>(a, m, most * BM, n, (uint64_t)GRID_MOST * BN);
+            const uint32_t tm = (uint32_t)((b.m + BM - 1) / BM);
+            linear_tile<T, O, BM, BN, WN, BK, ST, KG><<<tm * tn, 128 * WN * KG, 0, s>>>(b, tm, tn);
+        }
     }
     return hipGetLastError();
 }
@@ -459,22 +475,20 @@ hipError_t tile_of(const LinearArgs &a, hipStream_t s) {
 template <class T, class O, int MF>
 hipError_t rows_of(const LinearArgs &a, hipStream_t s) {
     // 8 waves: k 384 to 4096 within 0.1 us of the best of 4, 8 and 16
-    linear_rows<T, O, MF><<<(a.n + 15) / 16, ROW_WAVES * 64, 0, s>>>(a);
+    linear_rows<T, O, MF><<<(a.n - 1) / 16 + 1, ROW_WAVES * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 
 template <class T, class O>
 hipError_t linear_of(LinearArgs a, void *ws, hipStream_t s) {
     if (by_rows(a)) {
-        for (uint64_t m = 0; m < a.m; m += FEW_ROWS) {
-            LinearArgs b = a;
-            b.m = std::min(a.m - m, FEW_ROWS);
-            b.x = (const T *)a.x + m * a.ldx;
-            b.y = (O *)a.y + m * a.ldy;
-            if (a.residual) b.residual = (const O *)a.residual + m * a.ldr;
-            const hipError_t e = b.m <= 16 ? rows_of<T, O, 1>(b, s) : rows_of<T, O, 2>(b, s);
-            if (e != hipSuccess) return e;
-        }
+        static_assert(ROW_WAVES * 64 <= 1024, "GRID_MOST is for 1024 threads");
+        for (uint64_t n = 0; n < a.n; n += GRID_MOST * 16)
+            for (uint64_t m = 0; m < a.m; m += FEW_ROWS) {
+                const LinearArgs b = part_of<T, O>(a, m, FEW_ROWS, n, GRID_MOST * 16);
+                const hipError_t e = b.m <= 16 ? rows_of<T, O, 1>(b, s) : rows_of<T, O, 2>(b, s);
+                if (e != hipSuccess) return e;
+            }
         return hipSuccess;
     }
     const bool px = packs(a, a.x, a.ldx), pw = packs(a, a.w, a.ldw);

@@ -154,3 +154,16 @@ def test_linear_of_long_rows(ops, m, n, k):  # noqa: F811
     assert torch.equal(y, want.to(BF))
     del x, w
     torch.cuda.empty_cache()
+
+
+def test_linear_of_many_columns(ops):  # noqa: F811
+    """More columns than one launch's 2^32 threads reach."""
+    m, n = 2, 2 ** 27 + 40
+    say("linear, 2^27 + 40 columns")
+    w = (torch.arange(n, device="cuda") % 127).to(BF)[:, None]
+    x, b = torch.tensor([[1.0], [-2.0]], dtype=BF, device="cuda"), (torch.arange(n, device="cuda") % 3).to(BF)
+    r = torch.ones(m, n, dtype=BF, device="cuda")
+    y = ops.linear(x, w, bias=b, residual=r)
+    assert torch.equal(y, (x.float() * w[:, 0].float() + b.float() + 1).to(BF))  # exact in 32 bits
+    del w, b, r, y
+    torch.cuda.empty_cache()
