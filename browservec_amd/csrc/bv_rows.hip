@@ -7,9 +7,9 @@
 namespace bvk {
 namespace {
 
-// workgroups of a launch: a grid holds fewer than 2^32 threads a dimension, more
-// work is launched in pieces
-constexpr uint32_t GRID_MOST = 1u << 23;
+// workgroups of a launch: of 2^32 threads and more a dimension it runs the low 32
+// bits, so with up to 1024 a workgroup more work is launched in pieces
+constexpr uint32_t GRID_MOST = 1u << 21;
 
 // ---------------------------------------------------------------- rotary --
 // A thread turns (or copies) one unit of a token's heads: eight pairs, whose

@@ -167,3 +167,43 @@ def test_linear_of_many_columns(ops):  # noqa: F811
     assert torch.equal(y, (x.float() * w[:, 0].float() + b.float() + 1).to(BF))  # exact in 32 bits
     del w, b, r, y
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------- rows, sizes --
+def test_norm_of_more_rows_than_a_launch(ops):  # noqa: F811
+    """Rows of 16 waves, one a workgroup: 2^22 workgroups are 2^32 threads."""
+    rows, dim = 2 ** 22 + 100, 4104
+    say("norm of 2^22 + 100 rows")
+    if torch.cuda.mem_get_info()[0] < 2 * rows * dim + 2 ** 32:
+        pytest.skip("not enough device memory free")
+    x = torch.full((rows, dim), 3.0, dtype=BF, device="cuda")
+    ops.norm(x, kind="rms", out=x)  # 3 / sqrt(9 + 1e-5) is 1 in bfloat16
+    assert all((x[a:a + 2 ** 17] == 1).all() for a in range(0, rows, 2 ** 17))
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("mode", ["mean", "last"])
+def test_pool_of_more_sequences_than_a_launch(mode):
+    """The same of sequences, nearly all of them empty: the first and the last are not."""
+    from browservec_amd import DeviceContext, EmbedOps
+    from tests.helpers import need_gpu
+
+    need_gpu()
+    n, dim = 2 ** 22 + 100, 4104
+    say("pool of 2^22 + 100 sequences", mode)
+    if torch.cuda.mem_get_info()[0] < 8 * n * dim + 2 ** 32:  # the result and as many partial sums
+        pytest.skip("not enough device memory free")
+    ctx = DeviceContext(0)
+    e = EmbedOps(ctx)
+    x = torch.cat([torch.full((2, dim), 2.0), torch.full((3, dim), -5.0)]).to(BF).cuda()
+    cu = torch.full((n + 1,), 2, dtype=torch.int32, device="cuda")
+    cu[0], cu[-1] = 0, 5
+    y = torch.full((n, dim), 7.0, device="cuda")
+    e.pool(x, cu, mode=mode, unit=False, out=y)
+    assert (y[0] == 2).all() and (y[-1] == -5).all()
+    assert all((y[a:min(n - 1, a + 2 ** 17)] == 0).all() for a in range(1, n - 1, 2 ** 17))
+    del x, y, cu
+    torch.cuda.empty_cache()
+    e.destroy()
+    ctx.destroy()
