@@ -17,10 +17,13 @@ struct bv_embed {
     hipStream_t own = nullptr, stream = nullptr;
     void *zeros = nullptr;  // 256 bytes of zeros
     // Workspaces of each stream that needed one, the last of a stream's in
-    // use.  Smaller ones stay until the handle goes, since captured graphs hold
-    // their addresses; each is at least one and a half times the one before.
+    // use; a capture has its own, since its graph may run beside the stream's
+    // other work and other graphs.  All stay until the handle goes: kernels that
+    // still run, and graphs, hold their addresses.  Each is at least one and a
+    // half times the one before.
     struct Workspace {
         hipStream_t stream;
+        unsigned long long capture;  // 0: none
         void *p;
         size_t cap;
     };
@@ -36,20 +39,33 @@ int embed_live(bv_embed *e) {
 }
 
 int embed_workspace(bv_embed *e, size_t bytes, void **out) {
+    if (!bytes) return BV_OK;
+    unsigned long long capture = 0;
+    if (e->stream) {  // the null stream cannot be captured
+        hipStreamCaptureStatus status;
+        unsigned long long id = 0;
+        HIPX(e->dev, hipStreamGetCaptureInfo(e->stream, &status, &id), "workspace");
+        if (status == hipStreamCaptureStatusActive) capture = id + 1;
+    }
     size_t had = 0;
     for (size_t i = e->ws.size(); i-- && !had;)
-        if (e->ws[i].stream == e->stream) {
+        if (e->ws[i].stream == e->stream && e->ws[i].capture == capture) {
             had = e->ws[i].cap;
             *out = e->ws[i].p;
         }
     if (bytes <= had) return BV_OK;
-    bv_embed::Workspace w{e->stream, nullptr, (std::max(bytes, had + had / 2) + 4095) & ~size_t(4095)};
+    bv_embed::Workspace w{e->stream, capture, nullptr, (std::max(bytes, had + had / 2) + 4095) & ~size_t(4095)};
     try {
         e->ws.reserve(e->ws.size() + 1);
     } catch (const std::bad_alloc &) {
         return fail(BV_E_OOM, "out of host memory");
     }
-    HIPX(e->dev, hipMalloc(&w.p, w.cap), "workspace");
+    // an allocation is no part of a capture: only the relaxed mode lets it pass
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (capture) HIPX(e->dev, hipThreadExchangeStreamCaptureMode(&mode), "workspace");
+    const hipError_t err = hipMalloc(&w.p, w.cap);
+    if (capture) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    HIPX(e->dev, err, "workspace");
     e->ws.push_back(w);
     *out = w.p;
     return BV_OK;

@@ -347,8 +347,10 @@ int bv_graph_search_beams(bv_graph *g, const float *queries, uint32_t nq, const 
  * A handle is used by one thread at a time.  Its workspaces, one for each
  * stream it is used on, grow with the largest call so far and are held until
  * the handle is destroyed: after one call of a size on a stream, further calls
- * of it there allocate nothing and launch only kernels, so they can be
- * captured into a HIP graph. */
+ * of it there allocate nothing.  Calls launch only kernels and can be captured
+ * into a HIP graph.  Each capture has workspaces of its own, held until the
+ * handle is destroyed, so that graphs may run beside each other and beside
+ * other calls; runs of the same graph follow one another. */
 #define BV_F32 0
 #define BV_F16 1
 #define BV_BF16 2

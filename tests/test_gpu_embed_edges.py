@@ -207,3 +207,60 @@ def test_pool_of_more_sequences_than_a_launch(mode):
     torch.cuda.empty_cache()
     e.destroy()
     ctx.destroy()
+
+
+# ------------------------------------------------------------------- graphs --
+def test_graphs_run_beside_each_other(ops):  # noqa: F811
+    """Two graphs of calls that need workspaces, captured on one stream, replayed
+    on two streams at once, with eager calls on a third: none uses another's
+    workspace."""
+    say("graphs beside each other")
+
+    def calls(seed):
+        x, w = rand((700, 1003), seed, BF).cuda(), rand((500, 1003), seed + 1, BF, 0.05).cuda()  # packed rows
+        rows = rand((6000, 520), seed + 2, HF).cuda()  # partial sums
+        q, k, v = (rand((n, h, 64), seed + i, BF).cuda() for i, (n, h) in enumerate([(3, 8), (9000, 2), (9000, 2)], 3))  # split keys
+        cu, cq, ck = dev_cu([0, 2500, 6000]), dev_cu([0, 1, 3]), dev_cu([0, 4000, 9000])
+        return [lambda: ops.linear(x, w), lambda: ops.pool(rows, cu, kind="layer"),
+                lambda: ops.attention(q, k, v, cq, ck, max_q=2, max_k=5000)]
+
+    sets = [calls(10), calls(50), calls(90)]
+    want = [[f() for f in fns] for fns in sets]
+    torch.cuda.synchronize()
+    capture, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for fns in sets[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=capture):
+            outs.append([[f() for f in fns] for _ in range(4)])
+        graphs.append(g)
+    for _ in range(5):
+        for o in (t for out in outs for row in out for t in row):
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(capture):
+            eager = [[f() for f in sets[2]] for _ in range(4)]
+        torch.cuda.synchronize()
+        for out, w in zip(outs + [eager], want):
+            for row in out:
+                assert all(torch.equal(a, b) for a, b in zip(row, w))
+
+
+def test_a_capture_on_a_stream_without_calls_before(ops):  # noqa: F811
+    """Workspaces that a capture is the first to need."""
+    say("capture without calls before")
+    rows, cu = rand((5000, 264), 1, BF).cuda(), dev_cu([0, 5000])
+    want = ops.pool(rows, cu)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        out = ops.pool(rows, cu)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(ops.pool(rows, cu), want)
