@@ -139,7 +139,8 @@ __device__ __forceinline__ void row_alone(const AttentionArgs &a, const Attentio
         }
         const float best = fmaxf(top, wave_max(s));
         const float keep = top == best ? 1.0f : exp2f(top - best);
-        const float w = j + (int32_t)lane < seen ? exp2f(s - best) : 0.0f;
+        const float m = best == -INFINITY ? 0.0f : best;  // keys that score -inf weigh nothing, as in the tiles
+        const float w = j + (int32_t)lane < seen ? exp2f(s - m) : 0.0f;
         top = best;
         sum = sum * keep + wave_sum(w);
         ps[lane] = w;

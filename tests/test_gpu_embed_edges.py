@@ -264,3 +264,24 @@ def test_a_capture_on_a_stream_without_calls_before(ops):  # noqa: F811
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert torch.equal(ops.pool(rows, cu), want)
+
+
+# -------------------------------------------------------- attention, values --
+@pytest.mark.parametrize("nq,nk,low", [(200, 200, 100), (200, 200, 64), (8, 200, 190), (8, 3000, 2900), (40, 3000, 2900), (150, 150, 10)])
+def test_attention_of_keys_that_score_minus_infinity(ops, nq, nk, low):  # noqa: F811
+    """Keys at the front that weigh nothing, a value at the end that only the last
+    query sees and that is not finite: the other queries' results are those of the
+    finite keys."""
+    say("attention, scores of -inf", nq, nk, low)
+    hq, hk, d = 4, 2, 64
+    q, k, v = rand((nq, hq, d), 1, BF), rand((nk, hk, d), 2, BF), rand((nk, hk, d), 3, BF)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    k[:low, :, 0] = float("-inf")
+    v[-1, :, 5] = float("nan")
+    first = max(0, low - (nk - nq))  # the first query that sees a finite key
+    for hints in (dict(), dict(max_q=nq, max_k=nk)):
+        o = ops.attention(q.cuda(), k.cuda(), v.cuda(), dev_cu([0, nq]), dev_cu([0, nk]), **hints).cpu()
+        assert torch.isnan(o[:first]).all()  # 0 / 0
+        want, bound = attention_want(q[first:], k[low:], v[low:], [0, nq - first], [0, nk - low], True)
+        inside(o[first:-1], want[:-1], bound[:-1], f"scores of -inf {hints}")
+        assert torch.isnan(o[-1, :, 5]).all() and torch.isfinite(o[-1, :, :5]).all()
