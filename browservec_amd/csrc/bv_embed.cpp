@@ -87,20 +87,30 @@ bool fits(std::initializer_list<std::pair<uint64_t, uint64_t>> dims, uint64_t el
 }
 
 // The bytes an argument covers: `bytes` from p on, of them `width` at every
-// `pitch`.
+// `pitch`.  Heads have a second, finer pattern where tokens and heads lie at
+// multiples of the smaller stride.
 struct Span {
     const char *name;
     const void *p;
-    uint64_t bytes, pitch, width;
+    uint64_t bytes;
+    struct {
+        uint64_t pitch, width;
+    } at[2];
 };
-// Whether two arguments share memory.  Views of one buffer whose rows lie side
-// by side at the same pitch do not.
+// Whether two arguments share memory.  Views of one buffer whose rows, or heads,
+// lie side by side at the same pitch do not.
 bool overlap(const Span &a, const Span &b) {
     const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
     if (!a.bytes || !b.bytes || pa >= pb + b.bytes || pb >= pa + a.bytes) return false;
-    if (a.pitch != b.pitch || !a.pitch) return true;
-    const uint64_t d = pb >= pa ? (pb - pa) % a.pitch : (a.pitch - (pa - pb) % a.pitch) % a.pitch;
-    return d < a.width || d + b.width > a.pitch;
+    for (const auto &x : a.at)
+        for (const auto &y : b.at) {
+            // one piece fits any pitch
+            const uint64_t pitch = x.width == a.bytes ? y.pitch : y.width == b.bytes || x.pitch == y.pitch ? x.pitch : 0;
+            if (!pitch) continue;
+            const uint64_t d = pb >= pa ? (pb - pa) % pitch : (pitch - (pa - pb) % pitch) % pitch;
+            if (d >= x.width && d + y.width <= pitch) return false;
+        }
+    return true;
 }
 
 uint64_t size_of(uint32_t dtype) { return dtype == BV_F32 ? 4 : 2; }
@@ -123,8 +133,7 @@ int check_matrix(const char *what, Span &s, const void *p, uint64_t rows, uint64
     if (!fits({{rows, stride}, {cols, 1}}, elem, &s.bytes)) return fail(BV_E_INVALID, "%s: %s is too large", what, s.name);
     if (s.bytes && !p) return fail(BV_E_INVALID, "%s: %s is null", what, s.name);
     if ((uintptr_t)p % elem) return fail(BV_E_INVALID, "%s: %s is not aligned to its type", what, s.name);
-    s.pitch = stride * elem;
-    s.width = cols * elem;
+    s.at[0] = {stride * elem, cols * elem};
     return BV_OK;
 }
 
@@ -146,8 +155,13 @@ int check_heads(const char *what, Span &s, const void *p, uint64_t tokens, uint6
         return fail(BV_E_INVALID, "%s: %s is too large", what, s.name);
     if (s.bytes && !p) return fail(BV_E_INVALID, "%s: %s is null", what, s.name);
     if ((uintptr_t)p % elem) return fail(BV_E_INVALID, "%s: %s is not aligned to its type", what, s.name);
-    s.pitch = tokens_outer ? stride * elem : 0;
-    s.width = ((heads - 1) * head_stride + d) * elem;
+    if (tokens == 1 || heads == 1) {  // the other's stride alone
+        s.at[0] = {(heads == 1 ? stride : head_stride) * elem, d * elem};
+        return BV_OK;
+    }
+    const uint64_t outer = tokens_outer ? stride : head_stride, inner = tokens_outer ? head_stride : stride;
+    s.at[0] = {outer * elem, (((tokens_outer ? heads : tokens) - 1) * inner + d) * elem};
+    if (outer % inner == 0) s.at[1] = {inner * elem, d * elem};
     return BV_OK;
 }
 
@@ -295,12 +309,10 @@ extern "C" int bv_embed_rotary(bv_embed *e, const bv_embed_rotary_args *args) {
     }
     const bool q_in = a.q == a.q_out && a.q_stride == a.q_out_stride && a.q_head_stride == a.q_out_head_stride;
     const bool k_in = a.k == a.k_out && a.k_stride == a.k_out_stride && a.k_head_stride == a.k_out_head_stride;
-    // views of one buffer have interleaved extents: only outputs apart from
-    // their own input are told from it by extent
     if (!q_in) OK_OR_RETURN(check_apart("rotary", qo, {q}));
     if (!k_in) OK_OR_RETURN(check_apart("rotary", ko, {k}));
-    OK_OR_RETURN(check_apart("rotary", qo, {table, pos}));
-    OK_OR_RETURN(check_apart("rotary", ko, {table, pos}));
+    OK_OR_RETURN(check_apart("rotary", qo, {k, ko, table, pos}));
+    OK_OR_RETURN(check_apart("rotary", ko, {q, table, pos}));
     std::lock_guard<std::mutex> lock(e->mu);
     OK_OR_RETURN(embed_live(e));
     if (a.tokens == 0) return BV_OK;

@@ -285,3 +285,50 @@ def test_attention_of_keys_that_score_minus_infinity(ops, nq, nk, low):  # noqa:
         want, bound = attention_want(q[first:], k[low:], v[low:], [0, nq - first], [0, nk - low], True)
         inside(o[first:-1], want[:-1], bound[:-1], f"scores of -inf {hints}")
         assert torch.isnan(o[-1, :, 5]).all() and torch.isfinite(o[-1, :, :5]).all()
+
+
+# ------------------------------------------------------------------ rotary --
+FUSED = {  # a fused product's queries, keys and values as [tokens, heads, d] views
+    "tokens, 3, heads, d": lambda t, h, d: [x for x in rand((t, 3, h, d), 1, BF).cuda().unbind(1)],
+    "tokens, heads, 3 d": lambda t, h, d: rand((t, h, 3 * d), 1, BF).cuda().split(d, 2),
+    "tokens, heads, 3 d + 1": lambda t, h, d: rand((t, h, 3 * d + 1), 1, BF).cuda()[:, :, 1:].split(d, 2),
+    "heads, tokens, 3 d": lambda t, h, d: [x.transpose(0, 1) for x in rand((h, t, 3 * d), 1, BF).cuda().split(d, 2)],
+    "heads, 3, tokens, d": lambda t, h, d: [x.transpose(0, 1) for x in rand((h, 3, t, d), 1, BF).cuda().unbind(1)],
+    "tokens, 3 heads d + 5": lambda t, h, d: [x.unflatten(1, (h, d)) for x in rand((t, 3 * h * d + 5), 1, BF).cuda()[:, :3 * h * d].split(h * d, 1)],
+}
+
+
+@pytest.mark.parametrize("layout", FUSED)
+@pytest.mark.parametrize("tokens,heads", [(37, 4), (1, 4), (37, 1), (1, 1)])
+def test_rotary_of_fused_layouts_in_place(ops, layout, tokens, heads):  # noqa: F811
+    from browservec_amd import rotary_table
+
+    say("rotary in place", layout, tokens, heads)
+    table = torch.from_numpy(rotary_table(64, 16)).cuda()
+    q, k, v = FUSED[layout](tokens, heads, 32)
+    want = ops.rotary(q, k, table)
+    before = v.clone()
+    got = ops.rotary(q, k, table, out_q=q, out_k=k)
+    assert got[0] is q and torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, before)
+
+
+def test_rotary_outputs_that_overlap_are_refused(ops):  # noqa: F811
+    """Heads of queries and keys are turned in no order: neither output may be
+    the other's input or output."""
+    from browservec_amd import _lib as L
+    from browservec_amd import rotary_table
+
+    say("rotary outputs that overlap")
+    table = torch.from_numpy(rotary_table(64, 16)).cuda()
+    q, k, _ = FUSED["tokens, 3, heads, d"](9, 4, 32)
+    fused = rand((9, 5, 32), 2, BF).cuda()
+    own = torch.empty(9, 4, 32, dtype=BF, device="cuda")
+    before = [t.clone() for t in (q, k, fused)]
+    for kw in (dict(out_q=k), dict(out_k=q), dict(out_q=k, out_k=q), dict(out_q=own, out_k=own), dict(out_q=q, out_k=q)):
+        with pytest.raises(L.BVError) as e:
+            ops.rotary(q, k, table, **kw)
+        assert e.value.code == L.BV_E_INVALID and "overlaps" in str(e.value)
+    for kw in (dict(out_q=fused[:, :4]), dict(out_q=fused[:, 1:]), dict(out_k=fused[:, :4])):  # one head in common
+        with pytest.raises(L.BVError):
+            ops.rotary(fused[:, 1:] if "out_k" in kw else q, fused[:, :4] if "out_q" in kw else k, table, **kw)
+    assert all(torch.equal(a, b) for a, b in zip((q, k, fused), before))
