@@ -210,8 +210,9 @@ class EmbedOps:
         """softmax(scale q k^T) v of packed sequences: q [tokens, heads, d], k
         and v [keys, key heads, d] in float16 or bfloat16, cu_q and cu_k int32
         offsets [batch + 1] (cu_k None: cu_q).  causal: a sequence's last query
-        sees its last key.  max_q and max_k: the longest lengths where they are
-        known; they steer how the work is split."""
+        sees its last key.  scale None: 1 / sqrt(d); 0 is refused.  max_q and
+        max_k: the longest lengths where they are known; they steer how the
+        work is split."""
         a, address = self._attention
         if cu_k is None:
             cu_k = cu_q
@@ -237,6 +238,8 @@ class EmbedOps:
         a.tokens_q, a.heads_q, a.head_dim = sq
         a.tokens_k, a.heads_k, _ = sk
         a.max_q, a.max_k, a.scale = min(max_q, sq[0]), min(max_k, sk[0]), 0.0 if scale is None else scale
+        if scale is not None and a.scale == 0:  # in 32 bits; the library's word for its default
+            _bad(f"attention: scale {scale} is 0 in 32 bits")
         a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
         a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
         a.q_stride, a.q_head_stride, _ = q.stride()

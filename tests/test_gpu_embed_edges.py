@@ -332,3 +332,21 @@ def test_rotary_outputs_that_overlap_are_refused(ops):  # noqa: F811
         with pytest.raises(L.BVError):
             ops.rotary(fused[:, 1:] if "out_k" in kw else q, fused[:, :4] if "out_q" in kw else k, table, **kw)
     assert all(torch.equal(a, b) for a, b in zip((q, k, fused), before))
+
+
+# --------------------------------------------------------- attention, scale --
+def test_attention_scale_of_zero_is_refused(ops):  # noqa: F811
+    """Weights would all be equal; the library's 0 means the default."""
+    from browservec_amd import _lib as L
+
+    say("attention, scale 0")
+    q, cu = rand((4, 2, 8), 1, BF).cuda(), dev_cu([0, 4])
+    for scale in (0, 0.0, -0.0, 1e-60):
+        with pytest.raises(L.BVError) as e:
+            ops.attention(q, q, q, cu, scale=scale)
+        assert e.value.code == L.BV_E_INVALID and "scale" in str(e.value)
+    # as small as 32 bits hold: all weights equal
+    o = ops.attention(q, q, q, cu, causal=False, scale=1e-38)
+    want = q.cpu().double().mean(0, keepdim=True).expand(4, 2, 8)
+    inside(o, want, U[BF] * want.abs() * 1.01 + 2.0 ** -16, "equal weights")
+    assert torch.equal(ops.attention(q, q, q, cu, scale=None), ops.attention(q, q, q, cu, scale=8 ** -0.5))
