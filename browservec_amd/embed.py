@@ -35,6 +35,8 @@ def rotary_table(rows: int, rot_dim: int, base: float = 10000.0, scaling: str | 
         raise L.BVError(L.BV_E_INVALID, "rows and rot_dim are not negative")
     if scaling not in SCALINGS:
         raise L.BVError(L.BV_E_INVALID, f"unknown scaling {scaling!r}")
+    if magnitude == 0:  # the library's word for its default
+        raise L.BVError(L.BV_E_INVALID, "magnitude is 0")
     s = L.RotaryScaling(ctypes.sizeof(L.RotaryScaling), SCALINGS[scaling], base, factor, original_rows,
                         low_turns, high_turns, magnitude)
     out = np.empty((rows, rot_dim // 2, 2), np.float32)
