@@ -48,6 +48,13 @@ def _bad(msg: str):
     raise L.BVError(L.BV_E_INVALID, msg)
 
 
+def _counts(what: str, *sizes) -> None:
+    """Sizes that the library takes as 32 bits, which a ctypes field would cut
+    down to them without an error."""
+    if max(sizes) > 0xffffffff:
+        raise L.BVError(L.BV_E_UNSUPPORTED, f"{what}: a dimension of {max(sizes)} exceeds 32 bits")
+
+
 class EmbedOps:
     """Operators on one device, for one thread at a time.  Inputs whose last
     dimension is not contiguous, or whose rows overlap, are copied first."""
@@ -131,6 +138,7 @@ class EmbedOps:
         if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
             _bad("linear: x, weight and bias differ in type")
         n, k = sw
+        _counts("linear", n, k)
         flat = len(sx) == 2
         shape = (sx[0], n) if flat else (*sx[:-1], n)
         if out is None:
@@ -174,6 +182,7 @@ class EmbedOps:
             _bad("rotary: q and k are not [tokens, heads, d] alike")
         if len(st) != 3 or st[2] != 2 or table.dtype != self._f32 or not table.is_contiguous():
             _bad("rotary: the table is not contiguous float32 [rows, pairs, 2]")
+        _counts("rotary", sq[1], sq[2], 0 if k is None else k.shape[1], 2 * st[1], st[0])
         if positions is None:
             a.positions = None
         else:
@@ -225,6 +234,7 @@ class EmbedOps:
             _bad("attention: q is not [tokens, heads, d], or k and v are not [keys, key heads, d] alike")
         if k.dtype != dtype or v.dtype != dtype:
             _bad("attention: q, k and v differ in type")
+        _counts("attention", sq[1], sq[2], sk[1], cu_q.shape[0])
         cu_q = self._offsets(cu_q, "attention: cu_q")
         cu_k = self._offsets(cu_k, "attention: cu_k")
         if cu_q.shape != cu_k.shape or max_q < 0 or max_k < 0:
@@ -258,6 +268,7 @@ class EmbedOps:
             _bad(f"unknown norm {kind!r}")
         self._here(what, x, weight, bias, cu, out)
         dim = x.shape[-1]
+        _counts(what, dim, 0 if cu is None else cu.shape[0])
         a.weight = a.bias = None
         if weight is not None:
             weight = self._vector(weight, dim, "weight")

@@ -350,3 +350,32 @@ def test_attention_scale_of_zero_is_refused(ops):  # noqa: F811
     want = q.cpu().double().mean(0, keepdim=True).expand(4, 2, 8)
     inside(o, want, U[BF] * want.abs() * 1.01 + 2.0 ** -16, "equal weights")
     assert torch.equal(ops.attention(q, q, q, cu, scale=None), ops.attention(q, q, q, cu, scale=8 ** -0.5))
+
+
+# ------------------------------------------------------------------- counts --
+def test_dimensions_past_32_bits_are_refused(ops):  # noqa: F811
+    """Their low 32 bits would fit, and give part of a result.  (Expanded
+    tensors: nothing of the size is allocated.)"""
+    from browservec_amd import _lib as L
+
+    say("dimensions past 32 bits")
+    many = 2 ** 32 + 8
+    one, cu = torch.zeros(1, 1, dtype=BF, device="cuda"), dev_cu([0, 1])
+    heads = torch.zeros(1, 1, 1, dtype=BF, device="cuda")
+    table = torch.zeros(4, 0, 2, device="cuda")
+    for fn in (
+        lambda: ops.linear(one, one.expand(many, 1)),
+        lambda: ops.linear(one.expand(1, many), one.expand(1, many)),
+        lambda: ops.rotary(heads.expand(1, many, 1), None, table),
+        lambda: ops.rotary(heads, heads.expand(1, many, 1), table),
+        lambda: ops.rotary(heads.expand(1, 1, many), None, table),
+        lambda: ops.rotary(heads, None, torch.zeros(many, 0, 2, device="cuda")),
+        lambda: ops.attention(heads.expand(1, many, 1), heads, heads, cu, out=heads.expand(1, many, 1)),
+        lambda: ops.attention(heads, heads.expand(1, many, 1), heads.expand(1, many, 1), cu),
+        lambda: ops.attention(*(heads.expand(1, 1, many),) * 3, cu, out=heads.expand(1, 1, many)),
+        lambda: ops.norm(one.expand(1, many), out=one.expand(1, many)),
+        lambda: ops.pool(one.expand(1, many), cu, out=torch.zeros(1, 1, device="cuda").expand(1, many)),
+    ):
+        with pytest.raises(L.BVError) as e:
+            fn()
+        assert e.value.code == L.BV_E_UNSUPPORTED and "32 bits" in str(e.value)
