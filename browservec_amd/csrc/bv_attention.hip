@@ -741,6 +741,9 @@ bool few_rows(const AttentionArgs &a) {
     return queries * (a.hq / a.hk) <= 32 && a.d <= 128 && direct(a);
 }
 
+// Bytes of the partial results of one part of the keys.
+size_t part_bytes(const AttentionArgs &a) { return a.tq * a.hq * (a.d + 2) * 4; }
+
 // Parts of the keys, where tiles of rows alone leave most of the card idle:
 // chunks of one length over all sequences, so that each part is as much work,
 // as long as `wanted` workgroups or waves need for all of them.
@@ -754,7 +757,17 @@ uint32_t splits_of(const AttentionArgs &a, uint32_t *chunk) {
     uint64_t c = up(a.tk * (rows / a.batch) * a.hk / wanted);
     c = std::max<uint64_t>({c, few ? 128u : 256u, up((keys + MAX_SPLITS - 1) / MAX_SPLITS)});
     *chunk = (uint32_t)std::min<uint64_t>(c, 1u << 30);
-    return (uint32_t)std::max<uint64_t>(1, (keys + c - 1) / c);
+    uint64_t parts = std::max<uint64_t>(1, (keys + c - 1) / c);
+    // Where the longest length is not known, any sequence might have all keys, but
+    // most parts hold none where there are many sequences: as many as 256 MB of
+    // partial results are, or twice a sequence's share of the keys takes (64 x 12
+    // queries of 32 heads of 256, 600 keys each: 254 MB instead of 2.5 GB).  A
+    // sequence's last part takes what is left.
+    if (!a.max_k && a.batch > 1) {
+        const uint64_t part = part_bytes(a), share = (2 * a.tk / a.batch + c) / c;
+        parts = std::min(parts, std::max(share, (256u << 20) / part));
+    }
+    return (uint32_t)parts;
 }
 
 template <class T, int D, int GROUPS, bool DIRECT>
@@ -806,7 +819,7 @@ hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStre
 size_t attention_workspace(const AttentionArgs &a) {
     uint32_t chunk;
     const uint32_t splits = splits_of(a, &chunk);
-    return splits > 1 ? (size_t)splits * a.tq * a.hq * (a.d + 2) * 4 : 0;
+    return splits > 1 ? splits * part_bytes(a) : 0;
 }
 
 hipError_t launch_attention(const AttentionArgs &a, void *ws, hipStream_t s) {

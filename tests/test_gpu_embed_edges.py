@@ -379,3 +379,50 @@ def test_dimensions_past_32_bits_are_refused(ops):  # noqa: F811
         with pytest.raises(L.BVError) as e:
             fn()
         assert e.value.code == L.BV_E_UNSUPPORTED and "32 bits" in str(e.value)
+
+
+# ----------------------------------------------------- attention, workspace --
+def bidirectional_want(q, k, v, cu_q, cu_k):
+    """attention_want without a mask, its products on the GPU."""
+    u, group, scale = U[q.dtype], q.shape[1] // k.shape[1], q.shape[2] ** -0.5
+    out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    for a, e, ka, ke in zip(cu_q, cu_q[1:], cu_k, cu_k[1:]):
+        if e == a or ke == ka:
+            continue
+        for h in range(q.shape[1]):
+            qq, kk, vv = q[a:e, h].double(), k[ka:ke, h // group].double(), v[ka:ke, h // group].double()
+            s = scale * (qq @ kk.t().contiguous())
+            p = torch.exp(s - s.amax(1, keepdim=True))
+            total = p.sum(1, keepdim=True)
+            delta = (q.shape[2] + 2) * 2.0 ** -23 * scale * (qq.abs() @ kk.abs().t().contiguous()).amax(1, keepdim=True)
+            x = p @ vv / total
+            b = p @ vv.abs() / total * (u + 4 * delta + 2.0 ** -16 + 2 * (ke - ka) * 2.0 ** -24) + u * x.abs() * 1.01
+            if q.dtype == HF:
+                b += 2.0 ** -24 * (1 + vv.abs().sum(0, keepdim=True) / total)
+            out[a:e, h], bound[a:e, h] = x.cpu(), b.cpu()
+    return out, bound
+
+
+def test_attention_without_lengths_takes_little_memory():
+    """Parts of the keys are made for one sequence that might have all of them,
+    but not without end: 64 sequences of 600 keys, their lengths not said."""
+    from browservec_amd import DeviceContext, EmbedOps
+    from tests.helpers import need_gpu
+
+    need_gpu()
+    say("attention, workspace")
+    ctx = DeviceContext(0)
+    e = EmbedOps(ctx)
+    hq, hk, d = 32, 1, 256
+    cq, ck = cu_of([12] * 64), cu_of([600] * 64)
+    q, k, v = rand((cq[-1], hq, d), 1, BF, 1.5).cuda(), rand((ck[-1], hk, d), 2, BF).cuda(), rand((ck[-1], hk, d), 3, BF).cuda()
+    o, dq, dk = torch.empty_like(q), dev_cu(cq), dev_cu(ck)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    e.attention(q, k, v, dq, dk, causal=False, out=o)
+    torch.cuda.synchronize()
+    taken = free - torch.cuda.mem_get_info()[0]
+    inside(o, *bidirectional_want(q, k, v, cq, ck), "without lengths")
+    e.destroy()
+    ctx.destroy()
+    assert taken < 2 ** 28 + 2 ** 25, taken
