@@ -145,7 +145,7 @@ class EmbedOps:
             out = self._empty(shape, dtype=out_dtype or dtype, device=x.device)
         elif out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
             _bad(f"linear: out has shape {tuple(out.shape)}, not {tuple(shape)}, or another type")
-        y = out if flat else out.view(-1, n)
+        y = out if flat else _flat(out, "linear")
         a.dtype, a.out_dtype, a.activation = self._dtype(x, "linear"), self._dtype(out, "linear"), act
         x2, a.x_stride = _rows(x)
         w2, a.w_stride = _rows(weight)
@@ -267,6 +267,8 @@ class EmbedOps:
         if norm is None:
             _bad(f"unknown norm {kind!r}")
         self._here(what, x, weight, bias, cu, out)
+        if x.dim() < 1:
+            _bad(f"{what}: x has no dimension")
         dim = x.shape[-1]
         _counts(what, dim, 0 if cu is None else cu.shape[0])
         a.weight = a.bias = None
@@ -278,7 +280,7 @@ class EmbedOps:
             if weight is not None and weight.dtype != bias.dtype:
                 _bad(f"{what}: weight and bias differ in type")
             a.bias, a.weight_dtype = bias.data_ptr(), self._dtype(bias, what)
-        y = out if out.dim() == 2 else out.view(-1, dim)
+        y = out if out.dim() == 2 else _flat(out, what)
         a.dtype, a.out_dtype = self._dtype(x, what), self._dtype(out, what)
         a.y_stride = _out_stride(y, what)
         x2, a.x_stride = (y, a.y_stride) if out is x else _rows(x)
@@ -326,6 +328,14 @@ def _rows(t):
     if (one != 1 and n > 1) or (step < n and rows > 1):
         return t.contiguous(), 0
     return t, step if rows > 1 else 0
+
+
+def _flat(out, what: str):
+    """out [..., n] as rows of the same memory."""
+    try:
+        return out.view(-1, out.shape[-1])
+    except RuntimeError:
+        _bad(f"{what}: out's rows do not lie one stride apart")
 
 
 def _out_stride(y, what: str) -> int:

@@ -30,3 +30,13 @@ def test_outputs_that_do_not_overlap_pass():
     for out in (torch.empty(5, 2, 8), torch.empty(2, 5, 8).transpose(0, 1), torch.empty(5, 40)[:, 3:19].unflatten(1, (2, 8)),
                 torch.empty(1, 1, 8).expand(1, 1, 8)):
         embed._out_heads(out, "attention")
+
+
+def test_an_output_that_is_no_rows_at_one_stride_is_refused():
+    for out in (torch.empty(2, 5, 8).transpose(0, 1), torch.empty(4, 5, 8)[:, :3]):
+        with pytest.raises(L.BVError) as e:
+            embed._flat(out, "linear")
+        assert e.value.code == L.BV_E_INVALID
+    out = torch.empty(4, 5, 12)[:, :, 2:10]
+    rows = embed._flat(out, "linear")
+    assert rows.shape == (20, 8) and rows.data_ptr() == out.data_ptr() and embed._out_stride(rows, "linear") == 12

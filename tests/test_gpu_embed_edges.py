@@ -426,3 +426,28 @@ def test_attention_without_lengths_takes_little_memory():
     e.destroy()
     ctx.destroy()
     assert taken < 2 ** 28 + 2 ** 25, taken
+
+
+# ------------------------------------------------------------------- shapes --
+def test_shapes_of_other_than_two_dimensions(ops):  # noqa: F811
+    """Rows in any number of dimensions; outputs of theirs that are no rows at
+    one stride are refused, not left to torch."""
+    from browservec_amd import _lib as L
+
+    say("shapes")
+    x, w = rand((4, 5, 16), 1, BF).cuda(), rand((8, 16), 2, BF).cuda()
+    flat = ops.linear(x.flatten(0, 1), w)
+    y = torch.zeros(4, 5, 12, dtype=BF, device="cuda")
+    assert torch.equal(ops.linear(x, w, out=y[:, :, 2:10]).flatten(0, 1), flat)
+    assert torch.equal(ops.linear(x.transpose(0, 1), w).transpose(0, 1).flatten(0, 1), flat)
+    assert torch.equal(ops.linear(x[1, 2], w), flat[7])
+    n = ops.norm(x)
+    assert torch.equal(n, ops.norm(x.flatten(0, 1)).view(4, 5, 16)) and torch.equal(ops.norm(x[1, 2]), n[1, 2])
+    t = x.transpose(0, 1)
+    scalar = torch.zeros((), dtype=BF, device="cuda")
+    for fn in (lambda: ops.linear(x, w, out=torch.zeros(5, 4, 8, dtype=BF, device="cuda").transpose(0, 1)),
+               lambda: ops.linear(x, w, out=torch.zeros(4, 6, 8, dtype=BF, device="cuda")[:, :5]),
+               lambda: ops.norm(t, out=t), lambda: ops.norm(scalar), lambda: ops.linear(scalar, w)):
+        with pytest.raises(L.BVError) as e:
+            fn()
+        assert e.value.code == L.BV_E_INVALID
