@@ -14,6 +14,7 @@ that is an index's, and its appends and searches follow in order.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 
@@ -320,7 +321,7 @@ def _rows(t):
     """t [..., n] as rows and their stride: itself where the last dimension is
     contiguous and the others are one stride apart, or a copy.  0: packed."""
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     if t.is_contiguous():
         return t, 0
     rows, n = t.shape
@@ -333,7 +334,7 @@ def _rows(t):
 def _flat(out, what: str):
     """out [..., n] as rows of the same memory."""
     try:
-        return out.view(-1, out.shape[-1])
+        return out.view(math.prod(out.shape[:-1]), out.shape[-1])
     except RuntimeError:
         _bad(f"{what}: out's rows do not lie one stride apart")
 

@@ -40,3 +40,9 @@ def test_an_output_that_is_no_rows_at_one_stride_is_refused():
     out = torch.empty(4, 5, 12)[:, :, 2:10]
     rows = embed._flat(out, "linear")
     assert rows.shape == (20, 8) and rows.data_ptr() == out.data_ptr() and embed._out_stride(rows, "linear") == 12
+
+
+@pytest.mark.parametrize("shape,rows", [((2, 3, 0), 6), ((0,), 1), ((2, 0, 3), 0), ((4, 5, 8), 20), ((8,), 1)])
+def test_rows_of_no_elements(shape, rows):
+    assert embed._rows(torch.empty(shape))[0].shape == (rows, shape[-1])
+    assert embed._flat(torch.empty(shape), "linear").shape == (rows, shape[-1])

@@ -451,3 +451,12 @@ def test_shapes_of_other_than_two_dimensions(ops):  # noqa: F811
         with pytest.raises(L.BVError) as e:
             fn()
         assert e.value.code == L.BV_E_INVALID
+
+
+def test_sums_and_results_of_nothing(ops):  # noqa: F811
+    say("sums and results of nothing")
+    x, w, b = rand((2, 3, 16), 1, BF).cuda(), rand((8, 16), 2, BF).cuda(), rand((8,), 3, BF).cuda()
+    assert torch.equal(ops.linear(x[:, :, :0], w[:, :0], bias=b), b.expand(2, 3, 8))
+    assert ops.linear(x, w[:0]).shape == (2, 3, 0) and ops.linear(x[:, :0], w).shape == (2, 0, 8)
+    assert torch.equal(ops.linear(x[0, 0, :0], w[:, :0], bias=b), b)
+    assert ops.norm(x[:, :0]).shape == (2, 0, 16)
