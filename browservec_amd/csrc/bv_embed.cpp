@@ -137,14 +137,15 @@ int check_matrix(const char *what, Span &s, const void *p, uint64_t rows, uint64
     return BV_OK;
 }
 
-// Heads [tokens][heads][d], both strides filled in; of tokens and heads either
-// may be the outer one.
+// Heads [tokens][heads][d], both strides filled in, also those that a single
+// token or head leaves without a meaning; of tokens and heads either may be the
+// outer one.
 int check_heads(const char *what, Span &s, const void *p, uint64_t tokens, uint64_t heads, uint64_t d, uint64_t &stride,
                 uint64_t &head_stride, uint64_t elem) {
     s.p = p;
     if (tokens == 0 || heads == 0) return BV_OK;
-    if (head_stride == 0) head_stride = d;
-    if (stride == 0) stride = heads * head_stride;
+    if (head_stride == 0 || heads == 1) head_stride = d;
+    if (stride == 0 || tokens == 1) stride = heads * head_stride;
     const bool tokens_outer = head_stride >= d && (tokens <= 1 || stride >= (heads - 1) * head_stride + d);
     const bool heads_outer = stride >= d && (heads <= 1 || (unsigned __int128)head_stride >=
                                              (unsigned __int128)(tokens - 1) * stride + d);

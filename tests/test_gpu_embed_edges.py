@@ -460,3 +460,22 @@ def test_sums_and_results_of_nothing(ops):  # noqa: F811
     assert ops.linear(x, w[:0]).shape == (2, 3, 0) and ops.linear(x[:, :0], w).shape == (2, 0, 8)
     assert torch.equal(ops.linear(x[0, 0, :0], w[:, :0], bias=b), b)
     assert ops.norm(x[:, :0]).shape == (2, 0, 16)
+
+
+@pytest.mark.parametrize("tokens,heads,strides", [(1, 1, (1, 1, 1)), (1, 1, (3, 5, 1)), (1, 3, (2, 24, 1)), (6, 1, (24, 1, 1))])
+def test_strides_of_a_single_token_or_head(ops, tokens, heads, strides):  # noqa: F811
+    """They mean nothing, and a contiguous tensor may have any."""
+    from browservec_amd import rotary_table
+
+    say("strides of one", tokens, heads, strides)
+    d = 24
+    flat = [rand((200,), i, HF).cuda() for i in range(4)]
+    odd = [t.as_strided((tokens, heads, d), strides) for t in flat]
+    q, k, v = (t.clone(memory_format=torch.contiguous_format) for t in odd[:3])
+    cu = dev_cu([0, tokens])
+    want = ops.attention(q, k, v, cu)
+    assert torch.equal(ops.attention(*odd[:3], cu, out=odd[3]), want)
+    table = torch.from_numpy(rotary_table(8, 16)).cuda()
+    want = ops.rotary(q, k, table)
+    got = ops.rotary(*odd[:2], table, out_q=odd[0], out_k=odd[1])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
