@@ -479,3 +479,67 @@ def test_strides_of_a_single_token_or_head(ops, tokens, heads, strides):  # noqa
     want = ops.rotary(q, k, table)
     got = ops.rotary(*odd[:2], table, out_q=odd[0], out_k=odd[1])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------- paths of larger calls, both signs --
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,n,k", [(4096, 768, 768), (4100, 1030, 203), (6000, 1500, 264), (9000, 1400, 203), (8200, 4100, 520)])
+def test_linear_32_bit_results_of_large_tiles(ops, m, n, k, dtype):  # noqa: F811
+    """32-bit results and residuals out of tiles of 128 x 128 and 256 x 256."""
+    say("linear, 32-bit results", m, n, k, dtype)
+    x, w, b = rand((m, k), 1, dtype).cuda(), rand((n, k), 2, dtype, k ** -0.5).cuda(), rand((n,), 3, dtype).cuda()
+    r = rand((m, n), 4, F32).cuda()
+    y = ops.linear(x, w, bias=b, residual=r, activation="gelu_tanh", out_dtype=F32)
+    xd, wd, bd = x.double(), w.double(), b.double()
+    z = xd @ wd.t().contiguous() + bd
+    mag = xd.abs() @ wd.abs().t().contiguous() + bd.abs()
+    c = 2 * (2 / torch.pi) ** 0.5
+    want = z * torch.sigmoid(c * (z + 0.044715 * z ** 3)) + r.double()
+    bound = 1.13 * (k + 2) * 2.0 ** -23 * mag + 2.0 ** -20 * z.abs().clamp(min=1) + 2.0 ** -23 * want.abs()
+    inside(y, want.cpu(), (bound + U[F32] * (want.abs() + bound)).cpu(), "32-bit results")
+
+
+@pytest.mark.parametrize("scale", [-0.3, -1e-3])
+@pytest.mark.parametrize("d,dtype", [(64, BF), (80, HF), (17, BF), (128, HF), (200, BF)])
+@pytest.mark.parametrize("nq,nk", [([70, 0, 130], [70, 5, 200]), ([1, 3], [900, 40])])
+def test_attention_of_negative_scale(ops, nq, nk, d, dtype, scale):  # noqa: F811
+    """Queries change sign before the products; also in rows done one by one,
+    where a value that some do not see is not finite."""
+    say("attention, negative scale", nq, nk, d, dtype, scale)
+    cq, ck = cu_of(nq), cu_of(nk)
+    q, k, v = rand((cq[-1], 4, d), 1, dtype, 1.5), rand((ck[-1], 2, d), 2, dtype), rand((ck[-1], 2, d), 3, dtype)
+    want, bound = attention_want(q, k, v, cq, ck, True, scale=scale)
+    want_p, bound_p = attention_want(-q, k, v, cq, ck, True, scale=-scale)
+    assert torch.equal(want, want_p)  # the bound's sizes are those of the scores
+    args = [t.cuda() for t in (q, k, v)]
+    o = ops.attention(*args, dev_cu(cq), dev_cu(ck), scale=scale)
+    inside(o, want, bound_p, "negative scale")
+    assert torch.equal(o, ops.attention(-args[0], *args[1:], dev_cu(cq), dev_cu(ck), scale=-scale))
+    args[2][-1] = float("inf")
+    o = ops.attention(*args, dev_cu(cq), dev_cu(ck), scale=scale).cpu()
+    inside(o[:-1], want[:-1], bound_p[:-1], "negative scale, rows one by one")
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype", [(12, 12, 96, BF), (8, 8, 128, HF), (16, 4, 128, BF), (12, 4, 112, HF)])
+def test_attention_of_hundreds_of_short_texts(ops, hq, hk, d, dtype):  # noqa: F811
+    """Bidirectional, as an encoder's: more texts than compute units, of lengths
+    that end inside tiles, enough rows for the kernel of eight waves; a value that
+    is not finite stays in its text."""
+    lens = [(1, 17, 64, 65, 128, 200, 0, 333, 100, 256)[i % 10] for i in range(430)]
+    say("attention, short texts", hq, hk, d, dtype)
+    cu = cu_of(lens)
+    t = cu[-1]
+    q, k, v = rand((t, hq, d), 1, dtype, 1.5).cuda(), rand((t, hk, d), 2, dtype).cuda(), rand((t, hk, d), 3, dtype).cuda()
+    o = ops.attention(q, k, v, dev_cu(cu), causal=False)
+    want, bound = bidirectional_want(q, k, v, cu, cu)
+    inside(o, want, bound, "short texts")
+    assert torch.equal(o, ops.attention(q, k, v, dev_cu(cu), causal=False, max_q=max(lens), max_k=max(lens)))
+    s = 207  # 333 tokens
+    assert lens[s] == 333
+    v[cu[s] + 300, :, d // 2] = float("nan")
+    again = ops.attention(q, k, v, dev_cu(cu), causal=False)
+    same = torch.ones(t, dtype=torch.bool, device="cuda")
+    same[cu[s]:cu[s + 1]] = False
+    assert torch.equal(again[same], o[same])
+    mine = again[cu[s]:cu[s + 1]]
+    assert torch.isnan(mine[:, :, d // 2]).all() and torch.isfinite(mine[:, :, :d // 2]).all()
