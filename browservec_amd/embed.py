@@ -49,11 +49,10 @@ def _bad(msg: str):
     raise L.BVError(L.BV_E_INVALID, msg)
 
 
-def _counts(what: str, *sizes) -> None:
-    """Sizes that the library takes as 32 bits, which a ctypes field would cut
-    down to them without an error."""
-    if max(sizes) > 0xffffffff:
-        raise L.BVError(L.BV_E_UNSUPPORTED, f"{what}: a dimension of {max(sizes)} exceeds 32 bits")
+def _too_many(what: str, *sizes):
+    """Of sizes that the library takes as 32 bits: a ctypes field would cut them
+    down to these without an error."""
+    raise L.BVError(L.BV_E_UNSUPPORTED, f"{what}: a dimension of {max(sizes)} exceeds 32 bits")
 
 
 class EmbedOps:
@@ -139,7 +138,8 @@ class EmbedOps:
         if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
             _bad("linear: x, weight and bias differ in type")
         n, k = sw
-        _counts("linear", n, k)
+        if (n | k) >> 32:
+            _too_many("linear", n, k)
         flat = len(sx) == 2
         shape = (sx[0], n) if flat else (*sx[:-1], n)
         if out is None:
@@ -183,7 +183,9 @@ class EmbedOps:
             _bad("rotary: q and k are not [tokens, heads, d] alike")
         if len(st) != 3 or st[2] != 2 or table.dtype != self._f32 or not table.is_contiguous():
             _bad("rotary: the table is not contiguous float32 [rows, pairs, 2]")
-        _counts("rotary", sq[1], sq[2], 0 if k is None else k.shape[1], 2 * st[1], st[0])
+        hk = 0 if k is None else k.shape[1]
+        if (sq[1] | sq[2] | hk | 2 * st[1] | st[0]) >> 32:
+            _too_many("rotary", sq[1], sq[2], hk, 2 * st[1], st[0])
         if positions is None:
             a.positions = None
         else:
@@ -202,7 +204,7 @@ class EmbedOps:
             a.k, a.k_out, a.heads_k = None, None, 0
         else:
             ki, out_k = self._turned(k, out_k)
-            a.heads_k = k.shape[1]
+            a.heads_k = hk
             a.k, a.k_out = ki.data_ptr(), out_k.data_ptr()
             a.k_stride, a.k_head_stride, _ = ki.stride()
             a.k_out_stride, a.k_out_head_stride, _ = out_k.stride()
@@ -235,7 +237,8 @@ class EmbedOps:
             _bad("attention: q is not [tokens, heads, d], or k and v are not [keys, key heads, d] alike")
         if k.dtype != dtype or v.dtype != dtype:
             _bad("attention: q, k and v differ in type")
-        _counts("attention", sq[1], sq[2], sk[1], cu_q.shape[0])
+        if (sq[1] | sq[2] | sk[1] | cu_q.shape[0]) >> 32:
+            _too_many("attention", sq[1], sq[2], sk[1], cu_q.shape[0])
         cu_q = self._offsets(cu_q, "attention: cu_q")
         cu_k = self._offsets(cu_k, "attention: cu_k")
         if cu_q.shape != cu_k.shape or max_q < 0 or max_k < 0:
@@ -271,7 +274,8 @@ class EmbedOps:
         if x.dim() < 1:
             _bad(f"{what}: x has no dimension")
         dim = x.shape[-1]
-        _counts(what, dim, 0 if cu is None else cu.shape[0])
+        if (dim | (0 if cu is None else cu.shape[0])) >> 32:
+            _too_many(what, dim, 0 if cu is None else cu.shape[0])
         a.weight = a.bias = None
         if weight is not None:
             weight = self._vector(weight, dim, "weight")
