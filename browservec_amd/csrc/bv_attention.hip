@@ -228,12 +228,17 @@ __device__ __forceinline__ void store_rows(const AttentionArgs &a, const Attenti
 //     GROUPS 1 that share a CU fall into step, both waves of a SIMD multiplying
 //     and then both computing weights: 2300 cycles a tile and wave at D = 128
 //     where the products take 1024.)
-// Bound by the matrix cores and the vector unit together: at D = 128 they overlap
-// but for the turns' ends and the clock that the products leave (9001 and 16001
-// tokens, 8 heads over 2, causal, f16: 863 us, 1020 TFLOP/s), at D = 64 the
-// exponentials and their bookkeeping take longer than the products (96 x 1..512
-// tokens, 12 heads over 4, causal: 46 us, where the start of a workgroup also
-// counts).  With turns, D = 128 spills 2 registers a lane and D = 256 23.
+// At D = 128 (9001 and 16001 tokens, 8 heads over 2, causal, f16: 857 us, 1020
+// TFLOP/s; on another card 902) the matrix cores are busy for 53% of the cycles
+// and the vector unit, beside issuing to them, for 40%: the counters do not say
+// how much of that lies side by side, and so not whether the rest is turns or
+// waiting.  At D = 64 (96 x 1..512 tokens, 12 heads over 4: 46 us causal, 58
+// without a mask) they are busy for 12 and 38%: what is left is the chain at a
+// workgroup's start, offsets, queries and first keys one after the other.
+//   Registers spilled by a lane: with turns 2 at D = 128 and 23 at D = 256; where
+// not DIRECT 83 at D = 128 and 33 at D = 256.  4 x 4096 tokens, 8 heads, no mask:
+// d = 128 335 us, at odd addresses 749; d = 104 331, d = 100, whose elements are
+// loaded one by one, 2216; d = 256 1213, at odd addresses 2582.
 template <class T, int D, int KT, int GROUPS, bool DIRECT>
 __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {
@@ -445,6 +450,10 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= keep;
         }
+        // Weights are rounded to T here, as the second product takes them, while
+        // their sum has all bits: rounding errors of up to half a unit in T's last
+        // place a weight, averaged over the keys (2.6e-4 of the result's size in
+        // f16 against 2.0e-4 with weights of 32 bits, 1.9e-3 against 1.6e-3 in bf16).
         const float m = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int k = 0; k < KB; k++)
@@ -631,7 +640,7 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
                 for (int e = 0; e < 16; e++) o[d][e] *= keep;
         }
         const float m = top == -INFINITY ? 0.0f : top;
-        V w[2];
+        V w[2];  // rounded to T, as in attention_tile (bf16: 2.3e-3 against 1.6e-3)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[e], pl.c, -m));

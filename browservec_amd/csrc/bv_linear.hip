@@ -110,8 +110,9 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, uint64_t m, uint32_
 // Bound by the matrix cores where k is long (8192 x 8192 x 8192 bf16: 881 us, 1250
 // TFLOP/s; matrix instructions and barriers alone take 655 at the clock they leave),
 // and beside them by the epilogue where it is short: 32768 x 4096, k 1024, with
-// bias and GELU 327 us, 840 TFLOP/s, 66 of it the epilogue (the library's bare
-// product, without it, takes 218).  2037 x 768 x 768 (8.9 us): start, steps one
+// bias and GELU 316 to 327 us, 840 to 870 TFLOP/s (on another card 343, 802), 66 of
+// it the epilogue (the library's bare product, without it, takes 218); 335 with
+// results of 32 bits.  2037 x 768 x 768 (8.9 us): start, steps one
 // after the other and end of one round of tiles.
 //
 // LDS rows hold BK elements, in 16-byte chunks; chunk c of row r lies at
@@ -311,8 +312,9 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
 // --------------------------------------------------------------- few rows --
 // Up to 16 * MF rows of x (one question, a few): w is read once, straight into
 // the matrix instructions' registers, 16 of its rows a workgroup; the waves
-// split k and join their sums in LDS.  Bound by the read of w and by latency:
-// 32 x 4096 x 4096 14.2 us (33.6 MB), 9 x 384 x 1536 3.5.
+// split k and join their sums in LDS.  Bound by latency: a wave waits for four
+// steps' loads before it starts the next four, and 32 x 4096 x 4096 reads its 33.6
+// MB of w in 13.6 us, 2.5 TB/s; 9 x 384 x 1536 3.5, one chain.
 constexpr uint32_t ROW_WAVES = 8;
 template <class T, class O, int MF>
 __global__ __launch_bounds__(ROW_WAVES * 64) void linear_rows(LinearArgs a) {

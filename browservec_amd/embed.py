@@ -57,7 +57,10 @@ def _too_many(what: str, *sizes):
 
 class EmbedOps:
     """Operators on one device, for one thread at a time.  Inputs whose last
-    dimension is not contiguous, or whose rows overlap, are copied first."""
+    dimension is not contiguous, or whose rows overlap, are copied first.
+
+    Torch's autograd does not see these calls: results of tensors that require
+    gradients have none, and writes to ``out`` leave its version as it was."""
 
     def __init__(self, ctx):
         import torch

@@ -340,8 +340,9 @@ int bv_graph_search_beams(bv_graph *g, const float *queries, uint32_t nq, const 
  * waiting.  Matrices and heads have contiguous last dimensions and strides in
  * elements (0: packed); every alignment and size works, 16-byte aligned rows
  * run fastest.  Sums, softmax statistics and norms are 32-bit floats; results
- * are rounded once to the output's type, and the same call on the same inputs
- * gives the same bits.  Outputs may not overlap inputs except where a
+ * are rounded once to the output's type (in bv_embed_attention a key's weight
+ * as well, to the type of q, k and v, before it multiplies its value), and the
+ * same call on the same inputs gives the same bits.  Outputs may not overlap inputs except where a
  * description allows it.
  *
  * A handle is used by one thread at a time.  Its workspaces, one for each
@@ -514,7 +515,9 @@ int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *args);
  * clipped to the tokens there are) their mean, the first or the last of them,
  * and with unit divided by its 2-norm: the rows bv_index_append_device and the
  * queries bv_index_search_device take.  An empty sequence gives zeros, a
- * vector of norm zero stays as it is. */
+ * vector of norm zero stays as it is.  Squares are 32-bit floats too: the norms
+ * and the 2-norm are for elements whose squares, and their sum, are no larger
+ * than 3e38, and for rows whose sum of squares is above 1e-38. */
 #define BV_NORM_NONE 0
 #define BV_NORM_LAYER 1
 #define BV_NORM_RMS 2
