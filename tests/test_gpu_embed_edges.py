@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests.helpers import say
-from tests.test_gpu_embed import BF, F32, HF, U, attention_want, attention_want_gpu, cu_of, dev_cu, inside, linear_want, norm_want, ops, rand  # noqa: F401
+from tests.test_gpu_embed import BF, F32, HF, U, attention_want, cu_of, dev_cu, inside, linear_want, norm_want, ops, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
