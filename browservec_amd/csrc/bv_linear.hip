@@ -441,8 +441,8 @@ hipError_t pack(const void *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *t
     return hipGetLastError();
 }
 
-// A launch holds fewer than 2^32 threads, of more it runs the low 32 bits: so
-// many workgroups of at most 1024 at a time.
+// Workgroups of a launch: of 2^32 threads and more it runs the low 32 bits, so
+// with up to 1024 a workgroup more work is launched in pieces.
 constexpr uint32_t GRID_MOST = 1u << 21;
 
 // The part of a call that makes rows m to m + rows and columns n to n + cols.
