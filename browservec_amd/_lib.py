@@ -95,9 +95,15 @@ RotaryScaling = _args("RotaryScaling", """u32 size u32 kind f64 base f64 factor 
     f64 high_turns f64 magnitude""")
 AttentionArgs = _args("AttentionArgs", """u32 size u32 dtype u32 heads_q u32 heads_k u32 head_dim u32 causal u32 batch
     u32 max_q u32 max_k f32 scale u64 tokens_q u64 tokens_k ptr q ptr k ptr v ptr o ptr cu_q ptr cu_k u64 q_stride
-    u64 q_head_stride u64 k_stride u64 k_head_stride u64 v_stride u64 v_head_stride u64 o_stride u64 o_head_stride""")
+    u64 q_head_stride u64 k_stride u64 k_head_stride u64 v_stride u64 v_head_stride u64 o_stride u64 o_head_stride
+    u32 window u32 window_left u32 window_right u32 sinks""")
 NormArgs = _args("NormArgs", """u32 size u32 dtype u32 out_dtype u32 weight_dtype u32 norm u32 pool u32 unit u32 batch
     u32 dim f32 eps u64 tokens ptr x ptr weight ptr bias ptr cu ptr y u64 x_stride u64 y_stride""")
+LinearQ8Args = _args("LinearQ8Args", """u32 size u32 out_dtype u32 bias_dtype u32 activation u64 m u32 n u32 k ptr x ptr w
+    ptr x_scales ptr w_scales ptr bias ptr residual ptr y u64 x_stride u64 w_stride u64 residual_stride u64 y_stride""")
+AddNormArgs = _args("AddNormArgs", """u32 size u32 dtype u32 residual_dtype u32 out_dtype u32 weight_dtype u32 norm u32 dim
+    f32 eps u64 tokens ptr x ptr residual ptr weight ptr bias ptr total ptr y ptr scales u64 x_stride u64 residual_stride
+    u64 total_stride u64 y_stride""")
 
 vp = ctypes.c_void_p
 u32 = ctypes.c_uint32
@@ -153,10 +159,12 @@ SIGNATURES = {
     "bv_embed_stream": [vp, ctypes.POINTER(vp)],
     "bv_embed_sync": [vp],
     "bv_embed_linear": [vp, vp],
+    "bv_embed_linear_q8": [vp, vp],
     "bv_embed_rotary": [vp, vp],
     "bv_embed_rotary_table": [vp, u32, u32, vp, u64],
     "bv_embed_attention": [vp, vp],
     "bv_embed_norm": [vp, vp],
+    "bv_embed_add_norm": [vp, vp],
 }
 _RESTYPE = {"bv_last_error": ctypes.c_char_p}
 

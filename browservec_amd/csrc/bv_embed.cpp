@@ -1,10 +1,11 @@
 // Host side of the embedding operators declared in include/browservec_hip.h:
-// handles, argument checks, launches (bv_linear.hip, bv_attention.hip,
-// bv_rows.hip).
+// handles, argument checks, launches (bv_linear.hip, bv_linear_q8.hip,
+// bv_attention.hip, bv_attention_local.hip, bv_rows.hip, bv_add_norm.hip).
 #include "bv_embed.h"
 #include "bv_host.h"
 
 #include <cmath>
+#include <cstring>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -113,13 +114,17 @@ bool overlap(const Span &a, const Span &b) {
     return true;
 }
 
-uint64_t size_of(uint32_t dtype) { return dtype == BV_F32 ? 4 : 2; }
+uint64_t size_of(uint32_t dtype) { return dtype == BV_F32 ? 4 : dtype == BV_I8 ? 1 : 2; }
 
+// before: the size that an earlier, shorter form of the struct has; what it lacks
+// is 0.
 template <class A>
-int check_args(bv_embed *e, const A *given, A &a, const char *what) {
+int check_args(bv_embed *e, const A *given, A &a, const char *what, size_t before = sizeof(A)) {
     if (!e || !given) return fail(BV_E_INVALID, "%s: null argument", what);
-    if (given->size != sizeof(A)) return fail(BV_E_INVALID, "%s: args.size is %u, not %zu", what, given->size, sizeof(A));
-    a = *given;
+    if (given->size != sizeof(A) && given->size != before)
+        return fail(BV_E_INVALID, "%s: args.size is %u, not %zu", what, given->size, sizeof(A));
+    memset(&a, 0, sizeof(A));
+    memcpy(&a, given, given->size);
     return BV_OK;
 }
 
@@ -286,6 +291,57 @@ extern "C" int bv_embed_linear(bv_embed *e, const bv_embed_linear_args *args) {
     return BV_OK;
 }
 
+extern "C" int bv_embed_linear_q8(bv_embed *e, const bv_embed_linear_q8_args *args) {
+    bv_embed_linear_q8_args a;
+    OK_OR_RETURN(check_args(e, args, a, "linear_q8"));
+    if (a.out_dtype > BV_BF16 || (a.bias && a.bias_dtype > BV_BF16)) return fail(BV_E_UNSUPPORTED, "linear_q8: unknown dtype");
+    if (a.activation > BV_ACT_SILU) return fail(BV_E_INVALID, "linear_q8: unknown activation %u", a.activation);
+    if (a.k > LINEAR_Q8_MAX_K)
+        return fail(BV_E_UNSUPPORTED, "linear_q8: k %u exceeds %u, up to which sums of 32 bits are exact", a.k, LINEAR_Q8_MAX_K);
+    const uint64_t out = size_of(a.out_dtype);
+    Span x{"x"}, w{"w"}, sx{"x_scales"}, sw{"w_scales"}, b{"bias"}, r{"residual"}, y{"y"};
+    OK_OR_RETURN(check_matrix("linear_q8", x, a.x, a.m, a.k, a.x_stride, 1));
+    OK_OR_RETURN(check_matrix("linear_q8", w, a.w, a.n, a.k, a.w_stride, 1));
+    OK_OR_RETURN(check_matrix("linear_q8", y, a.y, a.m, a.n, a.y_stride, out));
+    uint64_t one = 0;
+    OK_OR_RETURN(check_matrix("linear_q8", sx, a.x_scales, 1, a.m, one, 4));
+    one = 0;
+    OK_OR_RETURN(check_matrix("linear_q8", sw, a.w_scales, 1, a.n, one, 4));
+    one = 0;
+    if (a.bias) OK_OR_RETURN(check_matrix("linear_q8", b, a.bias, 1, a.n, one, size_of(a.bias_dtype)));
+    if (a.residual) {
+        OK_OR_RETURN(check_matrix("linear_q8", r, a.residual, a.m, a.n, a.residual_stride, out));
+        const bool same = a.residual == a.y && a.residual_stride == a.y_stride;
+        if (!same) OK_OR_RETURN(check_apart("linear_q8", y, {r}));
+    }
+    OK_OR_RETURN(check_apart("linear_q8", y, {x, w, sx, sw, b}));
+    std::lock_guard<std::mutex> lock(e->mu);
+    OK_OR_RETURN(embed_live(e));
+    if (a.m == 0 || a.n == 0) return BV_OK;
+    LinearQ8Args l{};
+    l.out_dtype = (int)a.out_dtype;
+    l.act = (int)a.activation;
+    l.bias_dtype = (int)a.bias_dtype;
+    l.m = a.m;
+    l.n = a.n;
+    l.k = a.k;
+    l.x = (const int8_t *)a.x;
+    l.w = (const int8_t *)a.w;
+    l.x_scales = (const float *)a.x_scales;
+    l.w_scales = (const float *)a.w_scales;
+    l.bias = a.bias;
+    l.residual = a.residual;
+    l.y = a.y;
+    l.ldx = a.x_stride;
+    l.ldw = a.w_stride;
+    l.ldr = a.residual_stride;
+    l.ldy = a.y_stride;
+    void *ws = nullptr;
+    OK_OR_RETURN(embed_workspace(e, linear_q8_workspace(l), &ws));
+    HIPX(e->dev, launch_linear_q8(l, ws, e->stream), "linear_q8 kernel");
+    return BV_OK;
+}
+
 // ----------------------------------------------------------------- rotary --
 extern "C" int bv_embed_rotary(bv_embed *e, const bv_embed_rotary_args *args) {
     bv_embed_rotary_args a;
@@ -389,7 +445,8 @@ extern "C" int bv_embed_rotary_table(const bv_embed_rotary_scaling *scaling, uin
 // -------------------------------------------------------------- attention --
 extern "C" int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *args) {
     bv_embed_attention_args a;
-    OK_OR_RETURN(check_args(e, args, a, "attention"));
+    static_assert(offsetof(bv_embed_attention_args, window) == BV_EMBED_ATTENTION_ARGS_V1, "the struct's first form");
+    OK_OR_RETURN(check_args(e, args, a, "attention", BV_EMBED_ATTENTION_ARGS_V1));
     if (a.dtype != BV_F16 && a.dtype != BV_BF16)
         return fail(BV_E_UNSUPPORTED, "attention: dtype %u is not BV_F16 or BV_BF16", a.dtype);
     if (a.heads_q == 0 || a.heads_k == 0 || a.heads_q % a.heads_k)
@@ -446,6 +503,13 @@ extern "C" int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *ar
     t.so = a.o_stride;
     t.soh = a.o_head_stride;
     t.zeros = e->zeros;
+    if (a.window) {
+        t.left = std::min(a.window_left, 0x7fffffffu);
+        t.right = std::min(a.window_right, 0x7fffffffu);
+        t.sinks = std::min(a.sinks, 0x7fffffffu);
+        // a window that ends nowhere hides nothing
+        t.local = t.left < a.tokens_k || (!t.causal && t.right < std::max(a.tokens_q, a.tokens_k));
+    }
     void *ws = nullptr;
     OK_OR_RETURN(embed_workspace(e, attention_workspace(t), &ws));
     HIPX(e->dev, launch_attention(t, ws, e->stream), "attention kernel");
@@ -506,5 +570,66 @@ extern "C" int bv_embed_norm(bv_embed *e, const bv_embed_norm_args *args) {
         n.part = (float *)ws;
     }
     HIPX(e->dev, launch_norm(n, e->stream), "norm kernel");
+    return BV_OK;
+}
+
+extern "C" int bv_embed_add_norm(bv_embed *e, const bv_embed_add_norm_args *args) {
+    bv_embed_add_norm_args a;
+    OK_OR_RETURN(check_args(e, args, a, "add_norm"));
+    if (a.dtype > BV_BF16 || a.out_dtype > BV_I8 || ((a.weight || a.bias) && a.weight_dtype > BV_BF16))
+        return fail(BV_E_UNSUPPORTED, "add_norm: unknown dtype");
+    if (a.residual && a.residual_dtype != a.dtype && a.residual_dtype != BV_F32)
+        return fail(BV_E_UNSUPPORTED, "add_norm: residual_dtype %u is neither dtype nor BV_F32", a.residual_dtype);
+    if (a.norm > BV_NORM_RMS) return fail(BV_E_INVALID, "add_norm: unknown norm %u", a.norm);
+    if (a.dim == 0) return fail(BV_E_INVALID, "add_norm: dim is 0");
+    if (a.dim > NORM_MAX_DIM) return fail(BV_E_UNSUPPORTED, "add_norm: dim %u exceeds %u", a.dim, NORM_MAX_DIM);
+    if (a.norm && !(a.eps >= 0)) return fail(BV_E_INVALID, "add_norm: eps is negative");
+    if (a.total && !a.residual) return fail(BV_E_INVALID, "add_norm: total without a residual");
+    const bool codes = a.out_dtype == BV_I8;
+    const uint64_t in = size_of(a.dtype), added = size_of(a.residual_dtype), out = size_of(a.out_dtype), wt = size_of(a.weight_dtype);
+    Span x{"x"}, r{"residual"}, w{"weight"}, b{"bias"}, t{"total"}, y{"y"}, sc{"scales"};
+    OK_OR_RETURN(check_matrix("add_norm", x, a.x, a.tokens, a.dim, a.x_stride, in));
+    OK_OR_RETURN(check_matrix("add_norm", y, a.y, a.tokens, a.dim, a.y_stride, out));
+    if (a.residual) OK_OR_RETURN(check_matrix("add_norm", r, a.residual, a.tokens, a.dim, a.residual_stride, added));
+    if (a.total) OK_OR_RETURN(check_matrix("add_norm", t, a.total, a.tokens, a.dim, a.total_stride, added));
+    uint64_t one = 0;
+    if (a.weight) OK_OR_RETURN(check_matrix("add_norm", w, a.weight, 1, a.dim, one, wt));
+    one = 0;
+    if (a.bias) OK_OR_RETURN(check_matrix("add_norm", b, a.bias, 1, a.dim, one, wt));
+    one = 0;
+    if (codes) OK_OR_RETURN(check_matrix("add_norm", sc, a.scales, 1, a.tokens, one, 4));
+    const bool y_is_x = a.x == a.y && a.x_stride == a.y_stride && a.dtype == a.out_dtype;
+    const bool t_is_x = a.total == a.x && a.total_stride == a.x_stride && a.residual_dtype == a.dtype;
+    const bool t_is_r = a.total == a.residual && a.total_stride == a.residual_stride;
+    if (!y_is_x) OK_OR_RETURN(check_apart("add_norm", y, {x}));
+    OK_OR_RETURN(check_apart("add_norm", y, {r, w, b, t, sc}));
+    if (!t_is_x) OK_OR_RETURN(check_apart("add_norm", t, {x}));
+    if (!t_is_r) OK_OR_RETURN(check_apart("add_norm", t, {r}));
+    OK_OR_RETURN(check_apart("add_norm", t, {w, b, sc}));
+    OK_OR_RETURN(check_apart("add_norm", sc, {x, r, w, b}));
+    std::lock_guard<std::mutex> lock(e->mu);
+    OK_OR_RETURN(embed_live(e));
+    if (a.tokens == 0) return BV_OK;
+    AddNormArgs n{};
+    n.dtype = (int)a.dtype;
+    n.r_dtype = (int)a.residual_dtype;
+    n.out_dtype = (int)a.out_dtype;
+    n.wtype = (int)a.weight_dtype;
+    n.norm = (int)a.norm;
+    n.dim = a.dim;
+    n.eps = a.eps;
+    n.tokens = a.tokens;
+    n.x = a.x;
+    n.r = a.residual;
+    n.w = a.weight;
+    n.b = a.bias;
+    n.total = a.total;
+    n.y = a.y;
+    n.scales = (float *)a.scales;
+    n.ldx = a.x_stride;
+    n.ldr = a.residual_stride;
+    n.ldt = a.total_stride;
+    n.ldy = a.y_stride;
+    HIPX(e->dev, launch_add_norm(n, e->stream), "add_norm kernel");
     return BV_OK;
 }

@@ -1,5 +1,5 @@
-// Launchers of an embedding model's operators (bv_linear.hip, bv_attention.hip,
-// bv_rows.hip), called by bv_embed.cpp with checked arguments: every stride is
+// Launchers of an embedding model's operators (bv_linear.hip, bv_linear_q8.hip,
+// bv_attention.hip, bv_rows.hip, bv_add_norm.hip), called by bv_embed.cpp with checked arguments: every stride is
 // set, sizes fit the types below.  Strides are in elements.
 #pragma once
 
@@ -23,6 +23,23 @@ struct LinearArgs {
 size_t linear_workspace(const LinearArgs &a);
 hipError_t launch_linear(const LinearArgs &a, void *ws, hipStream_t s);
 
+// ------------------------------------------------------------- linear_q8 --
+// Sums of k products of codes, each at most 2^14, stay below 2^31.
+constexpr uint32_t LINEAR_Q8_MAX_K = 131071;
+struct LinearQ8Args {
+    int out_dtype, act, bias_dtype;
+    uint64_t m;
+    uint32_t n, k;
+    const int8_t *x, *w;
+    const float *x_scales, *w_scales;
+    const void *bias, *residual;
+    void *y;
+    uint64_t ldx, ldw, ldr, ldy;
+};
+// Bytes of workspace that a call needs (rows laid out for the matrix cores).
+size_t linear_q8_workspace(const LinearQ8Args &a);
+hipError_t launch_linear_q8(const LinearQ8Args &a, void *ws, hipStream_t s);
+
 // ------------------------------------------------------------- attention --
 struct AttentionArgs {
     int dtype, causal;
@@ -34,10 +51,13 @@ struct AttentionArgs {
     const int32_t *cu_q, *cu_k;
     uint64_t sq, sqh, sk, skh, sv, svh, so, soh;  // token and head strides
     const void *zeros;                            // 16 bytes of zeros
+    int local;  // a query sees `left` keys before its place, `right` after it and the first `sinks`
+    uint32_t left, right, sinks;                  // at most 2^31 - 1
 };
 // Bytes of workspace that a call needs (partial results of split keys).
 size_t attention_workspace(const AttentionArgs &a);
 hipError_t launch_attention(const AttentionArgs &a, void *ws, hipStream_t s);
+hipError_t launch_attention_local(const AttentionArgs &a, void *ws, hipStream_t s);
 
 // ------------------------------------------------------------------ rows --
 struct RotaryArgs {
@@ -67,5 +87,19 @@ struct NormArgs {
 // Workgroups that sum a chunk of one sequence's rows each: rows of NormArgs::part.
 uint64_t pool_chunks(uint64_t tokens, uint32_t batch);
 hipError_t launch_norm(const NormArgs &a, hipStream_t s);
+
+// Norm of x, or of x + r, to a float type or to codes of 8 bits and scales.
+enum { T_I8 = 3 };  // BV_I8
+struct AddNormArgs {
+    int dtype, r_dtype, out_dtype, wtype, norm;
+    uint32_t dim;
+    float eps;
+    uint64_t tokens;
+    const void *x, *r, *w, *b;
+    void *total, *y;
+    float *scales;
+    uint64_t ldx, ldr, ldt, ldy;
+};
+hipError_t launch_add_norm(const AddNormArgs &a, hipStream_t s);
 
 }  // namespace bvk

@@ -97,6 +97,13 @@ __device__ __forceinline__ float wave_max(float x) {
     BV_OVER_WAVE(x, fmaxf)
     return x;
 }
+// Of values without a sign the largest of their bits: infinity is above every
+// number, NaN above that.
+__device__ __forceinline__ float top_of(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+__device__ __forceinline__ float wave_top(float x) {
+    BV_OVER_WAVE(x, top_of)
+    return x;
+}
 #undef BV_OVER_WAVE
 // A lane's value and that of lane ^ 32.
 __device__ __forceinline__ float halves_sum(float x) {

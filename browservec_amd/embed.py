@@ -2,8 +2,10 @@
 
 The reference leaves text -> vector to another library
 (src/embed/transformers.ts); ``EmbedOps`` has the operators such a model's
-forward pass is made of (``linear``, ``rotary``, ``attention``, ``norm``), and
-``pool``, whose rows are what ``append_device`` and ``search_device`` take.
+forward pass is made of (``linear``, ``rotary``, ``attention``, ``norm``), in 8 bits
+as well (``norm_q8``, ``linear_q8``; ``add_norm`` where a product did not add its
+residual itself), and ``pool``, whose rows are what ``append_device`` and
+``search_device`` take.
 
 Inputs and outputs are torch tensors on the context's device; torch is only
 imported by this class.  Calls run on torch's current stream and return without
@@ -15,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import numpy as np
 
@@ -73,11 +76,12 @@ class EmbedOps:
         self._ordinal = ctx.ordinal
         self._dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self._int32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
+        self._int8, self._bf16 = torch.int8, torch.bfloat16
         # the arguments of each operator, filled in anew by every call, with
         # their address
-        self._linear, self._rotary, self._attention, self._norm = (
+        self._linear, self._rotary, self._attention, self._norm, self._linear_q8, self._add = (
             (t, ctypes.addressof(t)) for t in (c(ctypes.sizeof(c)) for c in (L.LinearArgs, L.RotaryArgs, L.AttentionArgs,
-                                                                             L.NormArgs)))
+                                                                             L.NormArgs, L.LinearQ8Args, L.AddNormArgs)))
         # the current stream as an int, without the object around it where torch has that
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current = raw or (lambda ordinal: torch.cuda.current_stream(ordinal).cuda_stream)
@@ -173,6 +177,61 @@ class EmbedOps:
         self._call(self.lib.bv_embed_linear, address)
         return out
 
+    def linear_q8(self, x, x_scales, weight, weight_scales, bias=None, residual=None, activation=None, out=None, out_dtype=None):
+        """act(x_scales weight_scales (x weight^T) + bias) + residual: x int8
+        [..., k] with a float32 scale a row (``norm_q8`` gives both), weight int8 [n,
+        k] with a scale a row ([n]; ``norm_q8`` with kind None), bias [n] of any float
+        type, residual and the result [..., n] of one float type: out_dtype, or out's
+        or residual's, or bfloat16.  k at most 131071."""
+        a, address = self._linear_q8
+        act = ACTIVATIONS.get(activation)
+        if act is None:
+            _bad(f"unknown activation {activation!r}")
+        self._here("linear_q8", x, x_scales, weight, weight_scales, bias, residual, out)
+        sx, sw, f32 = x.shape, weight.shape, self._f32
+        if len(sw) != 2 or len(sx) < 1 or sx[-1] != sw[1]:
+            _bad(f"linear_q8: x {tuple(sx)} and weight {tuple(sw)} do not fit")
+        if x.dtype != self._int8 or weight.dtype != self._int8:
+            _bad("linear_q8: x and weight are not int8")
+        if x_scales.shape != sx[:-1] or x_scales.dtype != f32:
+            _bad(f"linear_q8: x_scales are not float32 {tuple(sx[:-1])}")
+        n, k = sw
+        if (n | k) >> 32:
+            _too_many("linear_q8", n, k)
+        if weight_scales.dtype != f32:
+            _bad("linear_q8: weight_scales are not float32")
+        weight_scales, x_scales = self._vector(weight_scales, n, "linear_q8: weight_scales"), x_scales.contiguous()
+        flat = len(sx) == 2
+        shape = (sx[0], n) if flat else (*sx[:-1], n)
+        if out is None:
+            out = self._empty(shape, dtype=out_dtype or (self._bf16 if residual is None else residual.dtype), device=x.device)
+        elif out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+            _bad(f"linear_q8: out has shape {tuple(out.shape)}, not {tuple(shape)}, or another type")
+        y = out if flat else _flat(out, "linear_q8")
+        a.out_dtype, a.activation = self._dtype(out, "linear_q8"), act
+        x2, a.x_stride = _rows(x)
+        w2, a.w_stride = _rows(weight)
+        a.y_stride = _out_stride(y, "linear_q8")
+        a.m, a.n, a.k = x2.shape[0], n, k
+        a.x, a.w, a.y = x2.data_ptr(), w2.data_ptr(), y.data_ptr()
+        a.x_scales, a.w_scales = x_scales.data_ptr(), weight_scales.data_ptr()
+        if bias is None:
+            a.bias = None
+        else:
+            bias = self._vector(bias, n, "linear_q8: bias")
+            a.bias, a.bias_dtype = bias.data_ptr(), self._dtype(bias, "linear_q8: bias")
+        if residual is None:
+            a.residual = None
+        elif residual is out:
+            a.residual, a.residual_stride = a.y, a.y_stride
+        else:
+            if residual.shape != shape or residual.dtype != out.dtype:
+                _bad("linear_q8: residual differs from the result in shape or type")
+            residual, a.residual_stride = _rows(residual)
+            a.residual = residual.data_ptr()
+        self._call(self.lib.bv_embed_linear_q8, address)
+        return out
+
     def rotary(self, q, k, table, positions=None, interleaved: bool = False, out_q=None, out_k=None):
         """q [tokens, heads, d] and k (or None) with their first
         2 * table.shape[1] elements turned by the table's rows at each token's
@@ -223,13 +282,19 @@ class EmbedOps:
         return (x if out is x else _heads(x)), out
 
     def attention(self, q, k, v, cu_q, cu_k=None, max_q: int = 0, max_k: int = 0, causal: bool = True, scale: float | None = None,
-                  out=None):
+                  out=None, window=None, sinks: int = 0):
         """softmax(scale q k^T) v of packed sequences: q [tokens, heads, d], k
         and v [keys, key heads, d] in float16 or bfloat16, cu_q and cu_k int32
         offsets [batch + 1] (cu_k None: cu_q).  causal: a sequence's last query
         sees its last key.  scale None: 1 / sqrt(d); 0 is refused.  max_q and
         max_k: the longest lengths where they are known; they steer how the
-        work is split."""
+        work is split.
+
+        window (left, right): a query sees at most `left` keys before its place,
+        that at it and `right` after it (None: all on that side), and the
+        sequence's first `sinks` keys; query i's place is i + keys - queries of
+        its sequence.  causal hides what comes after a query's place, of the
+        first keys too."""
         a, address = self._attention
         if cu_k is None:
             cu_k = cu_q
@@ -257,6 +322,11 @@ class EmbedOps:
         a.tokens_q, a.heads_q, a.head_dim = sq
         a.tokens_k, a.heads_k, _ = sk
         a.max_q, a.max_k, a.scale = min(max_q, sq[0]), min(max_k, sk[0]), 0.0 if scale is None else scale
+        if window is None:
+            a.window = 0
+        else:
+            left, right = window
+            a.window, a.window_left, a.window_right, a.sinks = 1, _keys(left), _keys(right), _keys(sinks)
         if scale is not None and a.scale == 0:  # in 32 bits; the library's word for its default
             _bad(f"attention: scale {scale} is 0 in 32 bits")
         a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
@@ -307,6 +377,84 @@ class EmbedOps:
             _bad("norm: out differs from x in shape, or in type from out_dtype")
         return self._normed("norm", x, weight, bias, kind, eps, 0, False, None, out)
 
+    def _add_norm(self, what: str, x, residual, weight, bias, kind, eps, total, out, scales):
+        a, address = self._add
+        norm = NORMS.get(kind)
+        if norm is None:
+            _bad(f"unknown norm {kind!r}")
+        self._here(what, x, residual, weight, bias, total, out, scales)
+        dim = x.shape[-1]
+        if dim >> 32:
+            _too_many(what, dim)
+        a.weight = a.bias = a.residual = a.total = a.scales = None
+        if weight is not None:
+            weight = self._vector(weight, dim, "weight")
+            a.weight, a.weight_dtype = weight.data_ptr(), self._dtype(weight, what)
+        if bias is not None:
+            bias = self._vector(bias, dim, "bias")
+            if weight is not None and weight.dtype != bias.dtype:
+                _bad(f"{what}: weight and bias differ in type")
+            a.bias, a.weight_dtype = bias.data_ptr(), self._dtype(bias, what)
+        y = out if out.dim() == 2 else _flat(out, what)
+        a.dtype, a.y_stride = self._dtype(x, what), _out_stride(y, what)
+        t2 = None
+        if residual is not None:
+            if residual.shape != x.shape:
+                _bad(f"{what}: residual {tuple(residual.shape)} is not as x {tuple(x.shape)}")
+            if total is None:
+                total = self._empty(residual.shape, dtype=residual.dtype, device=x.device)
+            elif total.shape != residual.shape or total.dtype != residual.dtype:
+                _bad(f"{what}: total differs from the residual in shape or type")
+            a.residual_dtype = self._dtype(residual, what)
+            t2 = total if total.dim() == 2 else _flat(total, what)
+            a.total, a.total_stride = t2.data_ptr(), _out_stride(t2, what)
+            r2, a.residual_stride = (t2, a.total_stride) if total is residual else _rows(residual)
+            a.residual = r2.data_ptr()
+        elif total is not None:
+            _bad(f"{what}: total without a residual")
+        x2, a.x_stride = (y, a.y_stride) if out is x else (t2, a.total_stride) if total is x else _rows(x)
+        if scales is None:
+            a.out_dtype = self._dtype(out, what)
+        else:
+            a.out_dtype, a.scales = 3, scales.data_ptr()
+        a.norm, a.dim, a.eps, a.tokens, a.x, a.y = norm, dim, eps, x2.shape[0], x2.data_ptr(), y.data_ptr()
+        self._call(self.lib.bv_embed_add_norm, address)
+        return total
+
+    def add_norm(self, x, residual, weight=None, bias=None, kind: str = "layer", eps: float = 1e-5, total=None, out=None,
+                 out_dtype=None):
+        """The sum of x and residual [..., dim] and its norm (kind "layer", "rms" or
+        None) times weight plus bias, in one pass: the norm, and the sum rounded to
+        residual's type (x's or float32).  total: where the sum goes; residual itself
+        works, and x where it has that type.  out = x works in place."""
+        if x.dim() < 1:
+            _bad("add_norm: x has no dimension")
+        if residual is None:
+            _bad("add_norm: no residual")
+        if out is None:
+            out = self._empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        elif out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
+            _bad("add_norm: out differs from x in shape, or in type from out_dtype")
+        return out, self._add_norm("add_norm", x, residual, weight, bias, kind, eps, total, out, None)
+
+    def norm_q8(self, x, residual=None, weight=None, bias=None, kind: str | None = "layer", eps: float = 1e-5, total=None,
+                out=None, scales=None):
+        """The norm of x, or of its sum with residual as ``add_norm`` makes it, in 8
+        bits: int8 codes [..., dim], float32 scales [...] (the largest magnitude of a
+        row over 127; NaN, with codes 0, for a row that is not finite), and the sum, or
+        None without a residual.  kind None: the rows as they are, of weights too."""
+        if x.dim() < 1:
+            _bad("norm_q8: x has no dimension")
+        if out is None:
+            out = self._empty(x.shape, dtype=self._int8, device=x.device)
+        elif out.shape != x.shape or out.dtype != self._int8:
+            _bad("norm_q8: out differs from x in shape, or is not int8")
+        if scales is None:
+            scales = self._empty(x.shape[:-1], dtype=self._f32, device=x.device)
+        elif scales.shape != x.shape[:-1] or scales.dtype != self._f32 or not scales.is_contiguous():
+            _bad(f"norm_q8: scales are not contiguous float32 {tuple(x.shape[:-1])}")
+        return out, scales, self._add_norm("norm_q8", x, residual, weight, bias, kind, eps, total, out, scales)
+
     def pool(self, x, cu, mode: str = "mean", kind: str | None = None, weight=None, bias=None, eps: float = 1e-5,
              unit: bool = True, out=None):
         """One float32 vector per packed sequence of x [tokens, dim]: the mean,
@@ -322,6 +470,15 @@ class EmbedOps:
         elif out.shape != shape or out.dtype != self._f32:
             _bad(f"pool: out is not float32 {shape}")
         return self._normed("pool", x, weight, bias, kind, eps, pool, bool(unit), cu, out)
+
+
+def _keys(n) -> int:
+    """A number of keys for the library; None: all."""
+    if n is None:
+        return 0xffffffff
+    if n < 0:
+        _bad(f"attention: a window or a number of first keys of {n}")
+    return min(operator.index(n), 0xffffffff)
 
 
 def _rows(t):

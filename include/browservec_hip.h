@@ -355,6 +355,7 @@ int bv_graph_search_beams(bv_graph *g, const float *queries, uint32_t nq, const 
 #define BV_F32 0
 #define BV_F16 1
 #define BV_BF16 2
+#define BV_I8 3 /* codes of 8 bits, with a scale a row */
 
 typedef struct bv_embed bv_embed;
 
@@ -396,6 +397,35 @@ typedef struct bv_embed_linear_args {
     uint64_t y_stride;
 } bv_embed_linear_args;
 int bv_embed_linear(bv_embed *e, const bv_embed_linear_args *args);
+
+/* y = act(x_scales[i] w_scales[j] sum_k x[i][k] w[j][k] + bias[j]) + residual: x
+ * [m][k] and w [n][k] codes of 8 bits (bv_embed_add_norm makes them), a 32-bit
+ * float scale for each row of x and of w; bias [n] in bias_dtype (BV_F32, BV_F16
+ * or BV_BF16), residual and y [m][n] in out_dtype (of the three as well).  bias and
+ * residual may be NULL; residual may be y itself.  k is at most 131071: up to there
+ * the sums are exact in 32 bits; they are rounded to a 32-bit float and multiplied
+ * by x's scale, then by w's. */
+typedef struct bv_embed_linear_q8_args {
+    uint32_t size;        /* sizeof(bv_embed_linear_q8_args) */
+    uint32_t out_dtype;
+    uint32_t bias_dtype;
+    uint32_t activation;  /* BV_ACT_* */
+    uint64_t m;
+    uint32_t n;
+    uint32_t k;
+    const void *x;
+    const void *w;
+    const void *x_scales;
+    const void *w_scales;
+    const void *bias;
+    const void *residual;
+    void *y;
+    uint64_t x_stride;    /* elements from a row to the next; 0: packed */
+    uint64_t w_stride;
+    uint64_t residual_stride;
+    uint64_t y_stride;
+} bv_embed_linear_q8_args;
+int bv_embed_linear_q8(bv_embed *e, const bv_embed_linear_q8_args *args);
 
 /* Rotary positions: the first rot_dim elements of every head turn in pairs,
  * (a, b) -> (a cos - b sin, b cos + a sin); the others are copied.  Pairs are
@@ -472,7 +502,17 @@ int bv_embed_rotary_table(const bv_embed_rotary_scaling *scaling, uint32_t table
  * on it, whatever they hold.  scale 0: 1/sqrt(head_dim).  max_q and max_k are
  * the longest lengths as far as the caller knows them (0: unknown); they only
  * steer how the work is split, never which of it is done.  Queries outside
- * every sequence leave their rows of o as they are. */
+ * every sequence leave their rows of o as they are.
+ *
+ * With window, a query sees no more than the window_left keys before its place, the
+ * key at it, the window_right keys after it, and its sequence's first `sinks` keys
+ * (BV_ALL_KEYS or any number from 2^31 - 1 on: no end on that side).  The place of
+ * query i of lq is i + lk - lq among lk keys: the last query's is the last key.
+ * causal still hides all keys after a query's place, of the first keys too.  Keys
+ * that no query sees are not read.  Callers whose struct ends before `window` (size
+ * BV_EMBED_ATTENTION_ARGS_V1) have none. */
+#define BV_ALL_KEYS 0xffffffffu
+#define BV_EMBED_ATTENTION_ARGS_V1 168
 typedef struct bv_embed_attention_args {
     uint32_t size;        /* sizeof(bv_embed_attention_args) */
     uint32_t dtype;
@@ -500,6 +540,10 @@ typedef struct bv_embed_attention_args {
     uint64_t v_head_stride;
     uint64_t o_stride;
     uint64_t o_head_stride;
+    uint32_t window;      /* 0: none, and the three below mean nothing */
+    uint32_t window_left;
+    uint32_t window_right;
+    uint32_t sinks;
 } bv_embed_attention_args;
 int bv_embed_attention(bv_embed *e, const bv_embed_attention_args *args);
 
@@ -546,6 +590,41 @@ typedef struct bv_embed_norm_args {
     uint64_t y_stride;
 } bv_embed_norm_args;
 int bv_embed_norm(bv_embed *e, const bv_embed_norm_args *args);
+
+/* The sum t = x + residual (both [tokens][dim]; residual in residual_dtype, dtype
+ * or BV_F32) and its norm (BV_NORM_*, as bv_embed_norm) times weight plus bias, in
+ * one pass.  total, where it is not NULL, takes t rounded to residual_dtype; the
+ * norm is of t in 32 bits.  residual may be NULL (total is then, too): t = x.
+ * y [tokens][dim] in out_dtype; with BV_I8 the row's codes
+ *   q = round(y 127 / top), ties to even, with the scale top / 127 in scales
+ *   [tokens] (32-bit floats), top the row's largest |y|:
+ * what bv_embed_linear_q8 takes (weights too, with BV_NORM_NONE).  A row of zeros
+ * has scale 0; one that holds an infinity or NaN codes 0 and a scale of NaN.  total
+ * may be residual, or x where it has its type, and y may be x, each with the same
+ * strides and type. */
+typedef struct bv_embed_add_norm_args {
+    uint32_t size;        /* sizeof(bv_embed_add_norm_args) */
+    uint32_t dtype;
+    uint32_t residual_dtype;
+    uint32_t out_dtype;
+    uint32_t weight_dtype;
+    uint32_t norm;        /* BV_NORM_* */
+    uint32_t dim;
+    float eps;
+    uint64_t tokens;
+    const void *x;
+    const void *residual;
+    const void *weight;
+    const void *bias;
+    void *total;
+    void *y;
+    void *scales;         /* with BV_I8 alone */
+    uint64_t x_stride;    /* elements from a row to the next; 0: packed */
+    uint64_t residual_stride;
+    uint64_t total_stride;
+    uint64_t y_stride;
+} bv_embed_add_norm_args;
+int bv_embed_add_norm(bv_embed *e, const bv_embed_add_norm_args *args);
 
 #ifdef __cplusplus
 }
