@@ -35,6 +35,7 @@ struct LinearQ8Args {
     const void *bias, *residual;
     void *y;
     uint64_t ldx, ldw, ldr, ldy;
+    bool once;  // the launcher's: y goes past the caches
 };
 // Bytes of workspace that a call needs (rows laid out for the matrix cores).
 size_t linear_q8_workspace(const LinearQ8Args &a);

@@ -56,13 +56,14 @@ __device__ __forceinline__ void load8(const T *row, uint32_t at, uint32_t n, boo
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = early < 8 ? f[i] : 0.0f;
 }
-template <class T>
+template <bool ONCE = false, class T>
 __device__ __forceinline__ void store8(T *p, int n, const float (&f)[8]) {
     if (n >= 8) {
         typename Vec8<T>::type v;
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = (T)f[i];
-        *(typename Vec8<T>::unaligned *)p = v;
+        if (ONCE) __builtin_nontemporal_store(v, (typename Vec8<T>::unaligned *)p);
+        else *(typename Vec8<T>::unaligned *)p = v;
         return;
     }
 #pragma unroll
