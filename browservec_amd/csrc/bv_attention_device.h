@@ -122,9 +122,11 @@ __device__ __forceinline__ View rows_view(const AttentionArgs &a, const Place &p
 // -inf for the keys of a tile that the lane's row does not see.  Most tiles at the
 // window's ends are cut on one side.
 template <int KT>
-__device__ __forceinline__ void mask_local(const Tiles<KT> &tiles, int32_t t, const View &from, const View &to, const View &view,
-                                           uint32_t hi, v16f (&s)[KT / 32]) {
+__device__ __forceinline__ void mask_local(const Tiles<KT> &tiles, int32_t t, const View &from, const View &to, const AttentionArgs &a,
+                                           const Place &p, int32_t row, uint32_t group, uint32_t hi, v16f (&s)[KT / 32]) {
     if (tiles.all(t, from, to)) return;
+    // the row's view is made here, where it is rarely needed, not kept in registers
+    const View view = row < p.rows ? view_of(a, p, (uint32_t)row / group) : View{0, 0, 0};
     const int64_t k0 = (int64_t)tiles.key(t) + hi * 4;  // this lane's first key
     const bool firsts = t < tiles.firsts;
     const int32_t first = (int32_t)min((int64_t)view.first - k0, (int64_t)KT);
@@ -315,6 +317,41 @@ __device__ __forceinline__ void store_rows(const AttentionArgs &a, const Attenti
                     if (i + x < a.d) out[i + x] = f[x];
             }
         }
+}
+
+// The results of a wave's 32 rows from row wrow on, by rows: through 32 * D * 2
+// bytes of LDS at `lds`, the wave's own, so that a row leaves in pieces of 16 bytes
+// side by side, of whole chunks (d is a multiple of 8; store_rows' 8 bytes of 32 rows at a time took 20 us more of 6 x
+// 4001..8192 tokens with 12 heads of 64, 79 us in all).  Chunk c of row r lies at c ^
+// its swizzle.
+template <class T, int D>
+__device__ __forceinline__ void store_by_rows(const AttentionArgs &a, const Place &p, uint32_t group, uint32_t hk,
+                                              const v16f (&o)[D / 32], float sum, int32_t wrow, bool any, unsigned char *lds) {
+    typedef typename Vec8<T>::type V;
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    constexpr int CH = D / 8;
+    const uint32_t lane = threadIdx.x & 63, lo = lane & 31, hi = lane >> 5;
+    auto place = [&](uint32_t r, uint32_t c) { return r * D * 2 + ((c ^ (CH % 8 ? r & 3 : r & (CH - 1) & 15)) << 4); };
+    const float scale = 1.0f / halves_sum(sum);
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            V4 f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) f[x] = (T)(any ? o[d][e + x] * scale : 0.0f);
+            *(V4 *)(lds + place(lo, d * 4 + e / 4) + hi * 8) = f;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own rows
+#pragma unroll
+    for (int i = 0; i < 32 * CH / 64; i++) {
+        const uint32_t idx = i * 64 + lane, r = idx / CH, c = idx % CH;
+        const V f = *(const V *)(lds + place(r, c));
+        if (wrow + (int32_t)r >= p.rows || c * 8 >= a.d) continue;
+        const uint32_t at = wrow + r, query = at / group;
+        T *out = (T *)a.o + (p.qb + query) * a.so + (hk * group + at - query * group) * a.soh + c * 8;
+        *(typename Vec8<T>::unaligned *)out = f;
+    }
 }
 
 // 32 rows a wave; keys and values in tiles of KT, two of each in LDS, loaded
@@ -530,7 +567,7 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
     auto softmax = [&](int32_t t) {
         if (unseen(t)) return;
         if (LOCAL) {
-            mask_local<KT>(tiles, t, wfrom, wto, view, hi, s);
+            mask_local<KT>(tiles, t, wfrom, wto, a, p, row, group, hi, s);
         } else if ((t + 1) * KT > wfrom.hi) {
             const int32_t left = view.hi - t * KT - (int)hi * 4;  // keys that the row sees, from this lane's first
 #pragma unroll
@@ -632,6 +669,12 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
             row_alone<T, KT, LOCAL>(a, pl, p, group, hk, i, tiles, t0, t1, split, own, own + 256);
         return;
     }
+    if constexpr (LOCAL && DIRECT && 32 * D * 2 * 4 * GROUPS <= 4 * TILE) {
+        if (pl.splits == 1) {
+            store_by_rows<T, D>(a, p, group, hk, o, sum, wrow, in && view_of(a, p, query).any(), lds + wave * 32 * D * 2);
+            return;
+        }
+    }
     store_rows<T, D>(a, pl, o, top, sum, in, view.any(), token, head, split, t0 < t1);
 }
 
@@ -730,7 +773,7 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
 #pragma unroll
         for (int i = 0; i < D / 16; i++) s = mfma32(f[i], q[i], s);
         if (LOCAL) {
-            if (masked) mask_local<KT>(tiles, t, from, to, view, hi, reinterpret_cast<v16f(&)[1]>(s));
+            if (masked) mask_local<KT>(tiles, t, from, to, a, p, row, group, hi, reinterpret_cast<v16f(&)[1]>(s));
         } else if (masked) {
             const int32_t left = view.hi - t * KT - (int)hi * 4;
 #pragma unroll
@@ -864,22 +907,42 @@ bool few_rows(const AttentionArgs &a) {
 // Bytes of the partial results of one part of the keys.
 size_t part_bytes(const AttentionArgs &a) { return a.tq * a.hq * (a.d + 2) * 4; }
 
+// Parts of a window's keys.  A sequence's queries see a window's length, their own
+// number and the first ones.  Few rows a sequence: as many parts as fill the card
+// once (one of 32 rows and a key head is a wave's; by LDS a CU holds 4 waves at D = 128,
+// 8 at 64), of 128 keys or more.  A join takes 6 us, so that windows of 256 keys
+// are not split (13.4 us, split 13.3), nor, where each wave gets few parts, those
+// below 1024 (864 waves of 512 keys 23.6 us, split 31.6).  64 sequences of 4 x 4
+// heads of 64, windows of 4096: 116 us whole.
+uint32_t splits_of_window(const AttentionArgs &a, uint32_t *chunk) {
+    const uint64_t queries = a.max_q ? a.max_q : (a.tq + a.batch - 1) / a.batch;
+    const uint64_t most = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
+    auto up = [](uint64_t x, uint64_t to) { return (x + to - 1) / to * to; };
+    const uint64_t keys = std::min<uint64_t>(most, up(a.sinks, 32) + (uint64_t)a.left + (a.causal ? 0 : a.right) + queries);
+    const bool few = few_rows(a);
+    const uint64_t units = (a.tq * (a.hq / a.hk) / (few ? 32 : 128) + a.batch) * a.hk;
+    const uint64_t room = few ? 1024 * (a.d <= 32 ? 4 : a.d <= 64 ? 2 : 1) : 512;
+    *chunk = 0;
+    uint64_t parts = std::min(room / units, keys / (few ? 128 : 256));
+    if (parts < 2 || keys < (room / units < 8 ? 1024u : 384u)) return 1;
+    parts = std::min<uint64_t>({parts, MAX_SPLITS, std::max<uint64_t>(1, (256u << 20) / part_bytes(a))});
+    const uint64_t c = up((keys + parts - 1) / parts, few ? 32 : 128);
+    *chunk = (uint32_t)c;
+    return (uint32_t)((keys + c - 1) / c);
+}
+
 // Parts of the keys, where tiles of rows alone leave most of the card idle:
 // chunks of one length over all sequences, so that each part is as much work,
 // as long as `wanted` workgroups or waves need for all of them.
 uint32_t splits_of(const AttentionArgs &a, uint32_t *chunk) {
+    if (a.local) return splits_of_window(a, chunk);
     const bool few = few_rows(a);
     const uint64_t rows = a.tq * (a.hq / a.hk) / (few ? 32 : 128) + a.batch, wanted = few ? FEW_WAVES : 512;
-    uint64_t keys = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk, all = a.tk;
-    if (a.local) {  // of them a sequence's queries see a window's length, their own number and the first ones
-        const uint64_t queries = a.max_q ? a.max_q : (a.tq + a.batch - 1) / a.batch;
-        keys = std::min<uint64_t>(keys, (uint64_t)a.left + (a.causal ? 0 : a.right) + queries + a.sinks);
-        all = std::min<uint64_t>(all, keys * a.batch);
-    }
+    const uint64_t keys = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
     *chunk = 0;
     if (wanted / (rows * a.hk) < (few ? 4 : 2)) return 1;  // (few: joining costs what it saves)
     auto up = [](uint64_t x) { return (x + 127) / 128 * 128; };  // whole tiles, and not less than one of any kernel
-    uint64_t c = up(all * (rows / a.batch) * a.hk / wanted);
+    uint64_t c = up(a.tk * (rows / a.batch) * a.hk / wanted);
     c = std::max<uint64_t>({c, few ? 128u : 256u, up((keys + MAX_SPLITS - 1) / MAX_SPLITS)});
     *chunk = (uint32_t)std::min<uint64_t>(c, 1u << 30);
     uint64_t parts = std::max<uint64_t>(1, (keys + c - 1) / c);
@@ -889,7 +952,7 @@ uint32_t splits_of(const AttentionArgs &a, uint32_t *chunk) {
     // queries of 32 heads of 256, 600 keys each: 254 MB instead of 2.5 GB).  A
     // sequence's last part takes what is left.
     if (!a.max_k && a.batch > 1) {
-        const uint64_t part = part_bytes(a), share = (2 * all / a.batch + c) / c;
+        const uint64_t part = part_bytes(a), share = (2 * a.tk / a.batch + c) / c;
         parts = std::min(parts, std::max(share, (256u << 20) / part));
     }
     return (uint32_t)parts;
@@ -939,8 +1002,7 @@ hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStre
     return attention_sized<T, 256, true, LOCAL>(a, pl, s);
 }
 
-template <bool LOCAL>
-hipError_t launch_attention_as(const AttentionArgs &a, void *ws, hipStream_t s) {
+AttentionPlan plan_of(const AttentionArgs &a, void *ws) {
     AttentionPlan pl{};
     pl.c = std::fabs(a.scale) * 1.44269504f;
     pl.negate = a.scale < 0;
@@ -948,6 +1010,12 @@ hipError_t launch_attention_as(const AttentionArgs &a, void *ws, hipStream_t s) 
     pl.part_ml = (float2 *)ws;
     pl.part_o = (float *)ws + (size_t)pl.splits * a.tq * a.hq * 2;
     pl.zeros = a.zeros;
+    return pl;
+}
+
+template <bool LOCAL>
+hipError_t launch_attention_as(const AttentionArgs &a, void *ws, hipStream_t s) {
+    const AttentionPlan pl = plan_of(a, ws);
     return a.dtype == T_F16 ? attention_of<f16, LOCAL>(a, pl, s) : attention_of<bf16, LOCAL>(a, pl, s);
 }
 
