@@ -100,6 +100,7 @@ struct AddNormArgs {
     void *total, *y;
     float *scales;
     uint64_t ldx, ldr, ldt, ldy;
+    bool once;  // the launcher's: x and r are read past the caches
 };
 hipError_t launch_add_norm(const AddNormArgs &a, hipStream_t s);
 

@@ -76,7 +76,7 @@ class EmbedOps:
         self._ordinal = ctx.ordinal
         self._dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self._int32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
-        self._int8, self._bf16 = torch.int8, torch.bfloat16
+        self._int8, self._bf16, self._empty_like = torch.int8, torch.bfloat16, torch.empty_like
         # the arguments of each operator, filled in anew by every call, with
         # their address
         self._linear, self._rotary, self._attention, self._norm, self._linear_q8, self._add = (
@@ -204,7 +204,7 @@ class EmbedOps:
         flat = len(sx) == 2
         shape = (sx[0], n) if flat else (*sx[:-1], n)
         if out is None:
-            out = self._empty(shape, dtype=out_dtype or (self._bf16 if residual is None else residual.dtype), device=x.device)
+            out = self._empty(*shape, dtype=out_dtype or (self._bf16 if residual is None else residual.dtype), device=x.device)
         elif out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
             _bad(f"linear_q8: out has shape {tuple(out.shape)}, not {tuple(shape)}, or another type")
         y = out if flat else _flat(out, "linear_q8")
@@ -377,16 +377,23 @@ class EmbedOps:
             _bad("norm: out differs from x in shape, or in type from out_dtype")
         return self._normed("norm", x, weight, bias, kind, eps, 0, False, None, out)
 
+    def _like(self, x, dtype):
+        """A contiguous tensor of x's shape."""
+        if x.is_contiguous():  # a third of the time of one from a shape
+            return self._empty_like(x, dtype=dtype)
+        return self._empty(x.shape, dtype=dtype, device=x.device)
+
     def _add_norm(self, what: str, x, residual, weight, bias, kind, eps, total, out, scales):
         a, address = self._add
         norm = NORMS.get(kind)
         if norm is None:
             _bad(f"unknown norm {kind!r}")
         self._here(what, x, residual, weight, bias, total, out, scales)
-        dim = x.shape[-1]
+        shape = x.shape
+        dim = shape[-1]
         if dim >> 32:
             _too_many(what, dim)
-        a.weight = a.bias = a.residual = a.total = a.scales = None
+        a.weight = a.bias = None
         if weight is not None:
             weight = self._vector(weight, dim, "weight")
             a.weight, a.weight_dtype = weight.data_ptr(), self._dtype(weight, what)
@@ -395,26 +402,28 @@ class EmbedOps:
             if weight is not None and weight.dtype != bias.dtype:
                 _bad(f"{what}: weight and bias differ in type")
             a.bias, a.weight_dtype = bias.data_ptr(), self._dtype(bias, what)
-        y = out if out.dim() == 2 else _flat(out, what)
+        flat = len(shape) == 2
+        y = out if flat else _flat(out, what)
         a.dtype, a.y_stride = self._dtype(x, what), _out_stride(y, what)
         t2 = None
-        if residual is not None:
-            if residual.shape != x.shape:
-                _bad(f"{what}: residual {tuple(residual.shape)} is not as x {tuple(x.shape)}")
+        if residual is None:
+            if total is not None:
+                _bad(f"{what}: total without a residual")
+            a.residual = a.total = None
+        else:
+            if residual.shape != shape:
+                _bad(f"{what}: residual {tuple(residual.shape)} is not as x {tuple(shape)}")
             if total is None:
-                total = self._empty(residual.shape, dtype=residual.dtype, device=x.device)
-            elif total.shape != residual.shape or total.dtype != residual.dtype:
+                total = self._like(residual, residual.dtype)
+            elif total.shape != shape or total.dtype != residual.dtype:
                 _bad(f"{what}: total differs from the residual in shape or type")
-            a.residual_dtype = self._dtype(residual, what)
-            t2 = total if total.dim() == 2 else _flat(total, what)
-            a.total, a.total_stride = t2.data_ptr(), _out_stride(t2, what)
+            t2 = total if flat else _flat(total, what)
+            a.residual_dtype, a.total, a.total_stride = self._dtype(residual, what), t2.data_ptr(), _out_stride(t2, what)
             r2, a.residual_stride = (t2, a.total_stride) if total is residual else _rows(residual)
             a.residual = r2.data_ptr()
-        elif total is not None:
-            _bad(f"{what}: total without a residual")
         x2, a.x_stride = (y, a.y_stride) if out is x else (t2, a.total_stride) if total is x else _rows(x)
         if scales is None:
-            a.out_dtype = self._dtype(out, what)
+            a.out_dtype, a.scales = self._dtype(out, what), None
         else:
             a.out_dtype, a.scales = 3, scales.data_ptr()
         a.norm, a.dim, a.eps, a.tokens, a.x, a.y = norm, dim, eps, x2.shape[0], x2.data_ptr(), y.data_ptr()
@@ -432,7 +441,7 @@ class EmbedOps:
         if residual is None:
             _bad("add_norm: no residual")
         if out is None:
-            out = self._empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+            out = self._like(x, out_dtype or x.dtype)
         elif out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
             _bad("add_norm: out differs from x in shape, or in type from out_dtype")
         return out, self._add_norm("add_norm", x, residual, weight, bias, kind, eps, total, out, None)
@@ -446,11 +455,11 @@ class EmbedOps:
         if x.dim() < 1:
             _bad("norm_q8: x has no dimension")
         if out is None:
-            out = self._empty(x.shape, dtype=self._int8, device=x.device)
+            out = self._like(x, self._int8)
         elif out.shape != x.shape or out.dtype != self._int8:
             _bad("norm_q8: out differs from x in shape, or is not int8")
         if scales is None:
-            scales = self._empty(x.shape[:-1], dtype=self._f32, device=x.device)
+            scales = self._empty(x.shape[0] if x.dim() == 2 else x.shape[:-1], dtype=self._f32, device=x.device)
         elif scales.shape != x.shape[:-1] or scales.dtype != self._f32 or not scales.is_contiguous():
             _bad(f"norm_q8: scales are not contiguous float32 {tuple(x.shape[:-1])}")
         return out, scales, self._add_norm("norm_q8", x, residual, weight, bias, kind, eps, total, out, scales)
