@@ -201,9 +201,18 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
 
     // Results by rows: 32 of a wave's rows at a time go through LDS as 32-bit
     // floats, so that residuals are read and results written 16 bytes a lane
-    // along the rows.
+    // along the rows.  A lane's columns are the same in every row.
+    constexpr uint32_t LANES = WB / 8, RI = 64 / LANES;  // lanes of a row, rows of a turn
+    static_assert(64 % LANES == 0, "a lane keeps its columns");
     float *rows32 = (float *)lds + wave * 32 * PITCH;
-    const uint32_t nw = (wave >> 1) * WB, mr = (wave & 1) * (BM / 2);
+    const uint32_t mr = (wave & 1) * (BM / 2), lrow = lane / LANES, col = lane % LANES * 8, nc = (wave >> 1) * WB + col;
+    const int left = n0 + nc < a.n ? (int)min(8u, a.n - n0 - nc) : 0;
+    const uint32_t rows_left = left && m0 + mr < a.m ? (uint32_t)min((uint64_t)BM / 2, a.m - m0 - mr) : 0;
+    O *y = (O *)a.y + (m0 + mr + lrow) * a.ldy + n0 + nc;
+    const O *res = (const O *)a.residual + (a.residual ? (m0 + mr + lrow) * a.ldr + n0 + nc : 0);
+    float b[8], s[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) *(v4f *)(b + e) = *(const v4f *)(bias + nc + e), *(v4f *)(s + e) = *(const v4f *)(scale_w + nc + e);
 #pragma unroll
     for (int m = 0; m < MI; m++) {
         const float sx = scale_x[mr + m * 32 + lo];
@@ -211,30 +220,38 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
         for (int n = 0; n < NI; n++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const uint32_t col = n * 32 + q * 8 + hi * 4;
                 v4f f;
 #pragma unroll
                 for (int e = 0; e < 4; e++) f[e] = (float)acc[n][m][q * 4 + e] * sx;
-                *(v4f *)(rows32 + lo * PITCH + col) = f;
+                *(v4f *)(rows32 + lo * PITCH + n * 32 + q * 8 + hi * 4) = f;
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own rows
-        const uint64_t mw = m0 + mr + m * 32;
-        for (int i = 0; i < 32 * WB / 8 / 64; i++) {
-            const uint32_t idx = i * 64 + lane, row = idx / (WB / 8), col = idx % (WB / 8) * 8;
-            float f[8], b[8], s[8];
-            *(v4f *)f = *(const v4f *)(rows32 + row * PITCH + col);
-            *(v4f *)(f + 4) = *(const v4f *)(rows32 + row * PITCH + col + 4);
-            *(v4f *)b = *(const v4f *)(bias + nw + col);
-            *(v4f *)(b + 4) = *(const v4f *)(bias + nw + col + 4);
-            *(v4f *)s = *(const v4f *)(scale_w + nw + col);
-            *(v4f *)(s + 4) = *(const v4f *)(scale_w + nw + col + 4);
+#pragma unroll 4
+        for (uint32_t i = 0; i < 32 / RI; i++) {
+            float f[8];
+            const float *from = rows32 + (i * RI + lrow) * PITCH + col;
+            *(v4f *)f = *(const v4f *)from;
+            *(v4f *)(f + 4) = *(const v4f *)(from + 4);
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = fmaf(f[e], s[e], b[e]);
             activate8(f, a.act);
-            if (mw + row < a.m && n0 + nw + col < a.n) {
-                if (a.once) finish8<O, true>(a, mw + row, n0 + nw + col, f);
-                else finish8<O>(a, mw + row, n0 + nw + col, f);
+            if (m * 32 + i * RI + lrow < rows_left) {
+                if (a.residual) {
+                    if (left == 8) {
+                        float g[8];
+                        load8(res, g);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] += g[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] += (float)res[min(e, left - 1)];
+                    }
+                }
+                if (a.once) store8<true>(y, left, f);
+                else store8(y, left, f);
             }
+            y += RI * a.ldy;
+            res += RI * a.ldr;
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
