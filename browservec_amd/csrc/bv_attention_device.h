@@ -907,7 +907,7 @@ bool few_rows(const AttentionArgs &a) {
 // Bytes of the partial results of one part of the keys.
 size_t part_bytes(const AttentionArgs &a) { return a.tq * a.hq * (a.d + 2) * 4; }
 
-// Parts of a window's keys.  A sequence's queries see a window's length, their own
+// Parts of a window's keys.  A tile's queries see a window's length, their own
 // number and the first ones.  Few rows a sequence: as many parts as fill the card
 // once (one of 32 rows and a key head is a wave's; by LDS a CU holds 4 waves at D = 128,
 // 8 at 64), of 128 keys or more.  A join takes 6 us, so that windows of 256 keys
@@ -915,12 +915,12 @@ size_t part_bytes(const AttentionArgs &a) { return a.tq * a.hq * (a.d + 2) * 4; 
 // below 1024 (864 waves of 512 keys 23.6 us, split 31.6).  64 sequences of 4 x 4
 // heads of 64, windows of 4096: 116 us whole.
 uint32_t splits_of_window(const AttentionArgs &a, uint32_t *chunk) {
-    const uint64_t queries = a.max_q ? a.max_q : (a.tq + a.batch - 1) / a.batch;
+    const bool few = few_rows(a);
+    const uint64_t group = a.hq / a.hk, queries = std::min<uint64_t>(a.tq, ((few ? 32 : 128) + group - 1) / group);
     const uint64_t most = a.max_k ? std::min<uint64_t>(a.max_k, a.tk) : a.tk;
     auto up = [](uint64_t x, uint64_t to) { return (x + to - 1) / to * to; };
     const uint64_t keys = std::min<uint64_t>(most, up(a.sinks, 32) + (uint64_t)a.left + (a.causal ? 0 : a.right) + queries);
-    const bool few = few_rows(a);
-    const uint64_t units = (a.tq * (a.hq / a.hk) / (few ? 32 : 128) + a.batch) * a.hk;
+    const uint64_t units = (a.tq * group / (few ? 32 : 128) + a.batch) * a.hk;
     const uint64_t room = few ? 1024 * (a.d <= 32 ? 4 : a.d <= 64 ? 2 : 1) : 512;
     *chunk = 0;
     uint64_t parts = std::min(room / units, keys / (few ? 128 : 256));
@@ -1002,20 +1002,22 @@ hipError_t attention_of(const AttentionArgs &a, const AttentionPlan &pl, hipStre
     return attention_sized<T, 256, true, LOCAL>(a, pl, s);
 }
 
-AttentionPlan plan_of(const AttentionArgs &a, void *ws) {
+// The plan of a call whose keys are not split.
+AttentionPlan whole_plan(const AttentionArgs &a) {
     AttentionPlan pl{};
     pl.c = std::fabs(a.scale) * 1.44269504f;
     pl.negate = a.scale < 0;
-    pl.splits = splits_of(a, &pl.chunk);
-    pl.part_ml = (float2 *)ws;
-    pl.part_o = (float *)ws + (size_t)pl.splits * a.tq * a.hq * 2;
+    pl.splits = 1;
     pl.zeros = a.zeros;
     return pl;
 }
 
 template <bool LOCAL>
 hipError_t launch_attention_as(const AttentionArgs &a, void *ws, hipStream_t s) {
-    const AttentionPlan pl = plan_of(a, ws);
+    AttentionPlan pl = whole_plan(a);
+    pl.splits = splits_of(a, &pl.chunk);
+    pl.part_ml = (float2 *)ws;
+    pl.part_o = (float *)ws + (size_t)pl.splits * a.tq * a.hq * 2;
     return a.dtype == T_F16 ? attention_of<f16, LOCAL>(a, pl, s) : attention_of<bf16, LOCAL>(a, pl, s);
 }
 

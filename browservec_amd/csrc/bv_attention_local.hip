@@ -227,6 +227,11 @@ int window_tiles(const AttentionArgs &a) {
     return keys <= 160 ? 5 : a.d > 64 || (a.d <= 32 && !a.sinks) ? 9 : 0;
 }
 
+// (A tile's offsets within 64 rows have 32 bits.)
+bool by_window(const AttentionArgs &a) {
+    return direct(a) && std::max(a.sk, a.sv) < (1u << 22) && a.d <= 128 && !few_rows(a) && window_tiles(a);
+}
+
 template <class T, int D, int NT, bool FIRSTS>
 hipError_t window_of(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
     const uint32_t group = a.hq / a.hk;
@@ -260,8 +265,8 @@ hipError_t window_typed(const AttentionArgs &a, const AttentionPlan &pl, hipStre
 }  // namespace
 
 hipError_t launch_attention_local(const AttentionArgs &a, void *ws, hipStream_t s) {
-    if (direct(a) && std::max(a.sk, a.sv) < (1u << 22) && a.d <= 128 && !few_rows(a) && window_tiles(a)) {
-        const AttentionPlan pl = plan_of(a, nullptr);
+    if (by_window(a)) {
+        const AttentionPlan pl = whole_plan(a);
         return a.dtype == T_F16 ? window_typed<f16>(a, pl, s) : window_typed<bf16>(a, pl, s);
     }
     return launch_attention_as<true>(a, ws, s);

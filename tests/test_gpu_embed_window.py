@@ -227,3 +227,50 @@ def test_window_refusals_and_the_struct_before_it(ops):  # noqa: F811
     for size in (0, 160, 172, 176, 192):
         a.size = size
         assert lib.bv_embed_attention(ops.handle, ctypes.addressof(a)) == L.BV_E_INVALID
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype", [(2, 2, 64, BF), (6, 2, 64, HF), (8, 2, 96, BF), (7, 1, 128, HF), (3, 3, 128, BF), (4, 1, 32, BF),
+                                           (2, 2, 72, HF)])
+def test_short_windows(ops, hq, hk, d, dtype):  # noqa: F811
+    """Windows about the lengths at which a wave takes one tile of keys more or another
+    way: 160 and 288 keys of 32 rows; first keys up to 32 and one more."""
+    say("short windows", hq, hk, d, dtype)
+    cu = cu_of([700, 33, 128, 129, 1, 260])
+    q, k, v = rand((cu[-1], hq, d), 1, dtype, 1.5).cuda(), rand((cu[-1], hk, d), 2, dtype).cuda(), rand((cu[-1], hk, d), 3, dtype).cuda()
+    for causal, left, right, sinks in [(False, 64, 64, 0), (False, 64, 65, 1), (False, 140, 0, 32), (False, 0, 150, 33), (True, 128, 0, 4),
+                                       (True, 129, 5, 32), (False, 128, 128, 0), (False, 128, 129, 4), (True, 256, 0, 32), (True, 257, 0, 1),
+                                       (False, 270, 10, 31), (False, 300, 1, 0), (False, 5, 0, 20)]:
+        o = ops.attention(q, k, v, dev_cu(cu), causal=causal, window=(left, right), sinks=sinks)
+        inside(o, *window_want(q, k, v, cu, cu, causal, left, right, sinks), f"short window {causal} {left} {right} {sinks}")
+
+
+@pytest.mark.parametrize("nq,nk", [(1500, 1500), (900, 2000), (2000, 700)])
+@pytest.mark.parametrize("left,right,sinks", [(64, 64, 0), (100, 0, 4), (600, 0, 3)])
+def test_window_of_a_long_prompt_ignores_what_it_does_not_see(ops, nq, nk, left, right, sinks):  # noqa: F811
+    """One sequence and one head, whose keys would be split were the window longer; a
+    value that is not finite, which some rows see."""
+    say("window long unseen", nq, nk, left, right, sinks)
+    q, k, v = rand((nq, 1, 64), 1, BF).cuda(), rand((nk, 1, 64), 2, BF).cuda(), rand((nk, 1, 64), 3, BF).cuda()
+    seen = seen_of(nq, nk, right == 0, left, right, sinks)
+    want, bound = window_want(q, k, v, [0, nq], [0, nk], right == 0, left, right, sinks)
+    for bad in (0, nk // 2, nk - 1):
+        v2 = v.clone()
+        v2[bad, 0, 7] = float("nan")
+        o = ops.attention(q, k, v2, dev_cu([0, nq]), dev_cu([0, nk]), max_q=nq, max_k=nk, causal=right == 0, window=(left, right),
+                          sinks=sinks).cpu()
+        blind = ~seen[:, bad]
+        inside(o[blind], want[blind], bound[blind], f"unseen {bad}")
+        assert torch.isnan(o[~blind][:, 0, 7]).all() and torch.isfinite(o[~blind][:, 0, :7]).all()
+
+
+def test_window_of_many_texts(ops):  # noqa: F811
+    """More texts than a wave has lanes, of all lengths, and none at all between."""
+    say("window many texts")
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 300, (333,), generator=g).tolist()
+    cu = cu_of(lens)
+    for hq, hk, d in ((2, 1, 64), (3, 3, 32)):
+        q, k, v = rand((cu[-1], hq, d), 1, BF, 1.5).cuda(), rand((cu[-1], hk, d), 2, BF).cuda(), rand((cu[-1], hk, d), 3, BF).cuda()
+        for causal, left, right, sinks in ((False, 16, 30, 0), (True, 50, 0, 2)):
+            o = ops.attention(q, k, v, dev_cu(cu), causal=causal, window=(left, right), sinks=sinks, max_q=300)
+            inside(o, *window_want(q, k, v, cu, cu, causal, left, right, sinks), "many texts")
