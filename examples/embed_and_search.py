@@ -3,14 +3,16 @@ the embedding operators, the vectors it pools go into an index without leaving
 the device, and questions are embedded and searched the same way, all on the
 index's stream.
 
-    python examples/embed_and_search.py
+    python examples/embed_and_search.py [--q8] [--window TOKENS]
 
+--q8: the layers' products in 8 bits; --window: a token sees so many on both sides.
 The weights are random and the tokens are numbers: a real program loads a
 model's weights and its tokenizer's output in their place.
 """
 
 from __future__ import annotations
 
+import argparse
 import os
 import sys
 
@@ -25,12 +27,16 @@ from browservec_amd import DeviceContext, EmbedOps, FlatIndex, rotary_table  # n
 class Encoder:
     """A bidirectional encoder: embeddings, then layers of RMS norm, attention
     with rotary positions and grouped heads, and a wide layer, on a residual of
-    32-bit floats; the last norm, the mean and unit length make the vector."""
+    32-bit floats; the last norm, the mean and unit length make the vector.  q8: the
+    products of a layer take codes of 8 bits, of activations with a scale a token
+    and of weights with a scale a row.  window: how many tokens a token sees on each
+    side."""
 
     def __init__(self, ops: EmbedOps, vocab=1000, dim=384, layers=2, heads=6, key_heads=2, wide=1536, max_tokens=512,
-                 dtype=torch.bfloat16, seed=0):
+                 dtype=torch.bfloat16, seed=0, q8=False, window=None):
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.ops, self.heads, self.key_heads, self.d, self.dtype = ops, heads, key_heads, dim // heads, dtype
+        self.q8, self.window = q8, None if window is None else (window, window)
 
         def w(n, k):
             return (torch.randn(n, k, generator=g, device="cuda") * k ** -0.5).to(dtype)
@@ -41,6 +47,19 @@ class Encoder:
                             norm2=torch.ones(dim, device="cuda"), up=w(wide, dim), up_bias=torch.zeros(wide, device="cuda", dtype=dtype),
                             down=w(dim, wide)) for _ in range(layers)]
         self.last = torch.ones(dim, device="cuda")
+        # the weights of the products, in the form that they take
+        self.products = [{name: ops.norm_q8(layer[name], kind=None)[:2] if q8 else layer[name] for name in ("qkv", "out", "up", "down")}
+                         for layer in self.layers]
+
+    def norm(self, x, weight):
+        """The RMS norm, or x as it is (weight None), as a product takes it."""
+        kind = None if weight is None else "rms"
+        if self.q8:
+            return self.ops.norm_q8(x, weight=weight, kind=kind)[:2]
+        return x if weight is None else self.ops.norm(x, weight=weight, kind=kind, out_dtype=self.dtype)
+
+    def linear(self, x, weight, **kw):
+        return self.ops.linear_q8(*x, *weight, **kw) if self.q8 else self.ops.linear(x, weight, **kw)
 
     def __call__(self, sequences: list[list[int]]) -> torch.Tensor:
         """Unit vectors [len(sequences), dim] of lists of token ids."""
@@ -50,16 +69,14 @@ class Encoder:
         positions = torch.tensor([i for n in lens for i in range(n)], dtype=torch.int32, device="cuda")
         x = self.embeddings[tokens]  # the residual, 32 bits
         hq, hk, d = self.heads, self.key_heads, self.d
-        for layer in self.layers:
-            h = ops.norm(x, weight=layer["norm1"], kind="rms", out_dtype=self.dtype)
-            qkv = ops.linear(h, layer["qkv"])
+        for layer, w in zip(self.layers, self.products):
+            qkv = self.linear(self.norm(x, layer["norm1"]), w["qkv"], out_dtype=self.dtype)
             q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split([hq * d, hk * d, hk * d], 1))
             ops.rotary(q, k, self.table, positions=positions, out_q=q, out_k=k)
-            o = ops.attention(q, k, v, cu, max_q=max(lens), causal=False)
-            ops.linear(o.flatten(1), layer["out"], residual=x, out=x, out_dtype=torch.float32)
-            h = ops.norm(x, weight=layer["norm2"], kind="rms", out_dtype=self.dtype)
-            h = ops.linear(h, layer["up"], bias=layer["up_bias"], activation="gelu")
-            ops.linear(h, layer["down"], residual=x, out=x, out_dtype=torch.float32)
+            o = ops.attention(q, k, v, cu, max_q=max(lens), causal=False, window=self.window)
+            self.linear(self.norm(o.flatten(1), None), w["out"], residual=x, out=x, out_dtype=torch.float32)
+            h = self.linear(self.norm(x, layer["norm2"]), w["up"], bias=layer["up_bias"], activation="gelu", out_dtype=self.dtype)
+            self.linear(self.norm(h, None), w["down"], residual=x, out=x, out_dtype=torch.float32)
         return ops.pool(x, cu, kind="rms", weight=self.last)
 
 
@@ -74,10 +91,14 @@ def search(index, queries: torch.Tensor, k: int):
 
 
 def main() -> None:
+    parser = argparse.ArgumentParser()
+    parser.add_argument("--q8", action="store_true", help="the layers' products in 8 bits")
+    parser.add_argument("--window", type=int, help="how many tokens a token sees on each side")
+    args = parser.parse_args()
     ctx = DeviceContext(0)
     ops = EmbedOps(ctx)
     index = FlatIndex(ctx, 384, "cosine")
-    encoder = Encoder(ops)
+    encoder = Encoder(ops, q8=args.q8, window=args.window)
     torch.cuda.synchronize()  # the weights, made on torch's own stream
     r = np.random.default_rng(1)
     passages = [r.integers(0, 1000, r.integers(5, 200)).tolist() for _ in range(2000)]
