@@ -346,13 +346,19 @@ __global__ __launch_bounds__(ROW_WAVES * 64) void linear_q8_rows(LinearQ8Args a)
 
 // ---------------------------------------------------------------- packing --
 // Rows for linear_q8_tile, which loads 16 bytes at 16-byte addresses: k rounded
-// up to 16 with zeros.
-__global__ __launch_bounds__(256) void pack_codes(const int8_t *x, uint64_t ldx, uint32_t k, uint32_t chunks, uint64_t count, int8_t *y) {
+// up to 16 with zeros.  x's and w's in one launch (114 x 1000, k 820: 9.9 us, in two 12.1).
+struct PackJob {
+    const int8_t *from;
+    int8_t *to;
+    uint64_t ld, count;  // chunks of 16 codes in all
+};
+__global__ __launch_bounds__(256) void pack_codes(PackJob a, PackJob b, uint32_t k, uint32_t chunks) {
     const uint64_t step = (uint64_t)gridDim.x * 256;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += step) {
-        const uint64_t row = i / chunks;
+    for (uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x; n < a.count + b.count; n += step) {
+        const PackJob &j = n < a.count ? a : b;
+        const uint64_t i = n < a.count ? n : n - a.count, row = i / chunks;
         const uint32_t at = (uint32_t)(i - row * chunks) * 16;
-        const int8_t *p = x + row * ldx + at;
+        const int8_t *p = j.from + row * j.ld + at;
         union {
             int8_t b[16];
             v4i v;
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(256) void pack_codes(const int8_t *x, uint64_t ldx,
                 u.b[e] = at + e < k ? z : 0;
             }
         }
-        *(v4i *)(y + i * 16) = u.v;
+        *(v4i *)(j.to + i * 16) = u.v;
     }
 }
 
@@ -382,15 +388,6 @@ bool packs(const LinearQ8Args &a, const void *p, uint64_t ld) {
     return a.m > FEW_ROWS && a.k && (a.k % 16 || !aligned(p, ld) || ld >= FAR_ROWS);
 }
 uint64_t packed_bytes(uint64_t rows, uint32_t k) { return (rows * ((k + 15) / 16) * 16 + 255) & ~255ull; }
-
-hipError_t pack(const int8_t *&p, uint64_t &ld, uint64_t rows, uint32_t k, void *to, hipStream_t s) {
-    const uint32_t chunks = (k + 15) / 16;
-    const uint64_t count = rows * chunks;
-    pack_codes<<<(uint32_t)std::min<uint64_t>((count + 255) / 256, 8192), 256, 0, s>>>(p, ld, k, chunks, count, (int8_t *)to);
-    p = (const int8_t *)to;
-    ld = (uint64_t)chunks * 16;
-    return hipGetLastError();
-}
 
 // Workgroups of a launch: of 2^32 threads and more it runs the low 32 bits, so
 // with up to 1024 a workgroup more work is launched in pieces.
@@ -444,14 +441,22 @@ hipError_t linear_q8_of(LinearQ8Args a, void *ws, hipStream_t s) {
         }
         return hipSuccess;
     }
-    const bool px = packs(a, a.x, a.ldx), pw = packs(a, a.w, a.ldw);
-    if (px) {
-        const hipError_t e = pack(a.x, a.ldx, a.m, a.k, ws, s);
-        if (e != hipSuccess) return e;
-        ws = (char *)ws + packed_bytes(a.m, a.k);
-    }
-    if (pw) {
-        const hipError_t e = pack(a.w, a.ldw, a.n, a.k, ws, s);
+    const uint32_t chunks = (a.k + 15) / 16;
+    PackJob jobs[2] = {};
+    int n = 0;
+    auto pack = [&](const int8_t *&p, uint64_t &ld, uint64_t rows) {
+        if (!packs(a, p, ld)) return;
+        jobs[n++] = {p, (int8_t *)ws, ld, rows * chunks};
+        p = (const int8_t *)ws;
+        ld = (uint64_t)chunks * 16;
+        ws = (char *)ws + packed_bytes(rows, a.k);
+    };
+    pack(a.x, a.ldx, a.m);
+    pack(a.w, a.ldw, a.n);
+    if (n) {
+        const uint64_t count = jobs[0].count + jobs[1].count;
+        pack_codes<<<(uint32_t)std::min<uint64_t>((count + 255) / 256, 8192), 256, 0, s>>>(jobs[0], jobs[1], a.k, chunks);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     a.k = (a.k + 15) / 16 * 16;
