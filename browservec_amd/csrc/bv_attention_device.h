@@ -374,10 +374,13 @@ __device__ __forceinline__ void store_by_rows(const AttentionArgs &a, const Plac
 // waiting.  At D = 64 (96 x 1..512 tokens, 12 heads over 4: 46 us causal, 58
 // without a mask) they are busy for 12 and 38%: what is left is the chain at a
 // workgroup's start, offsets, queries and first keys one after the other.
-//   Registers spilled by a lane: with turns 2 at D = 128 and 23 at D = 256; where
-// not DIRECT 83 at D = 128 and 33 at D = 256.  4 x 4096 tokens, 8 heads, no mask:
-// d = 128 335 us, at odd addresses 749; d = 104 331, d = 100, whose elements are
-// loaded one by one, 2216; d = 256 1213, at odd addresses 2582.
+//   Registers spilled by a lane: with turns 3 at D = 128 and 23 at D = 256 (with a
+// window 17 and 28, outside the loop's common path).  4 x 4096 tokens, 8 heads, no
+// mask: d = 128 344 us, at odd addresses 791; d = 104 330, d = 100, whose elements are
+// loaded one by one, 1453; d = 256 1229, at odd addresses 2714.
+//   A window: 32768 tokens, 8 heads of 128 over 2, the last 4096 keys and 4 first ones, f16,
+// 573 to 612 us by card, 840 to 900 TFLOP/s of visible pairs; 6% more are computed, in tiles
+// that the window cuts and the first keys' own.
 template <class T, int D, int KT, int GROUPS, bool DIRECT, bool LOCAL>
 __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {
@@ -684,7 +687,7 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile
 // its way; no barriers.  Neighbouring waves take the key heads side by side in
 // memory.  Bound by the read of keys and values and the start of their chain:
 // 8 sequences of up to 32768 keys, 4 key heads of 64, one new token each: 25 us, and
-// 6 to join.
+// 6 to join; 64 sequences that see 4100 keys each 52, 4.7 TB/s, and 6.
 template <class T, int D, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, AttentionPlan pl, uint64_t first, uint64_t units) {
     typedef typename Vec8<T>::type V;
@@ -913,7 +916,7 @@ size_t part_bytes(const AttentionArgs &a) { return a.tq * a.hq * (a.d + 2) * 4; 
 // 8 at 64), of 128 keys or more.  A join takes 6 us, so that windows of 256 keys
 // are not split (13.4 us, split 13.3), nor, where each wave gets few parts, those
 // below 1024 (864 waves of 512 keys 23.6 us, split 31.6).  64 sequences of 4 x 4
-// heads of 64, windows of 4096: 116 us whole.
+// heads of 64, windows of 4096: 116 us whole, in 7 parts 59, in 22 64.
 uint32_t splits_of_window(const AttentionArgs &a, uint32_t *chunk) {
     const bool few = few_rows(a);
     const uint64_t group = a.hq / a.hk, queries = std::min<uint64_t>(a.tq, ((few ? 32 : 128) + group - 1) / group);

@@ -13,6 +13,10 @@ namespace {
 // three waits for memory (offsets; queries and keys; values) and none a tile, no
 // running maximum, no rescaling.  A wave's tiles begin at its own first key, so that
 // it computes no more of the neighbours' keys than fill its last one.
+//   Bound by the waits and HBM: 6 x 4001..8192 tokens, 12 heads of 64, 64 on both sides, 57
+// us, 3.8 TB/s of 5.1 that a copy reaches (vector unit busy for 42% of the cycles, matrix
+// cores for 11; attention_tile 79).  Four workgroups a CU: with keys and values in LDS side by side
+// there are two, 71; weights made tile by tile, which saves registers, 63.
 // FIRSTS: the sequence's first 32 keys, of which `sinks` count, are a tile of their
 // own; a key of the window counts there alone.
 template <class T, int D, int NT, bool FIRSTS>

@@ -35,6 +35,16 @@ __device__ __forceinline__ float bias_at(const LinearQ8Args &a, uint32_t n) {
 // multiplies those of the 32 before, and waits for the next tile before it
 // multiplies a tile's last 32, already in registers.
 //
+// Bound by the card's power and the end of a tile.  8192 x 8192 x 8192: 460 to 480 us,
+// 2.3 POP/s (the library's bare product 453): the matrix cores are busy for 60% of the cycles
+// at 1.8 GHz; without loads 385, without LDS reads as well 324.  32768 x 4096, k 1024,
+// bf16: the loop takes 127 us, all of it 168 (the library's bare product 195), with
+// bias and GELU 200, of which the activation's 13 instructions a result are 30 to 50.  20011 x
+// 1024, k 4096, onto a residual of 32 bits 122: 1.6 rounds of tiles.  Tried and slower:
+// groups of waves that take turns between LDS and matrix cores (482), four waves of 128 x 128 (539),
+// 192 x 128 tiles two a CU (535); steps of 64 codes ask the L2 for half lines and are
+// bound by its requests (580), but two such workgroups a CU cover each other's ends.
+//
 // LDS rows hold BK codes, in 16-byte chunks; chunk c of row r lies at
 // c ^ swizzle(r), so that sixteen lanes that read the same chunk of consecutive
 // rows cover all banks (256 bytes).  Loads put lane i's chunk at a fixed place, so the
@@ -115,6 +125,19 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[n][m][e] = 0;
 
+    // where this lane's results go
+    constexpr uint32_t LANES = WB / 8, RI = 64 / LANES;  // lanes of a row, rows of a turn
+    static_assert(64 % LANES == 0, "a lane keeps its columns");
+    const uint32_t mr = (wave & 1) * (BM / 2), lrow = lane / LANES, col = lane % LANES * 8, nc = (wave >> 1) * WB + col;
+    const int left = n0 + nc < a.n ? (int)min(8u, a.n - n0 - nc) : 0;
+    const uint32_t rows_left = left && m0 + mr < a.m ? (uint32_t)min((uint64_t)BM / 2, a.m - m0 - mr) : 0;
+    const O *res = (const O *)a.residual + (a.residual ? (m0 + mr + lrow) * a.ldr + n0 + nc : 0);
+    // Small tiles take their residuals to registers during the first step: there is
+    // nothing else to wait beside (2037 x 768, k 768, tiles of 64 x 128: 7.2 us, later 8.2).
+    constexpr uint32_t TURNS = MI * 32 / RI;
+    constexpr bool EARLY = ST == 2 && TURNS <= 4;
+    typename Vec8<O>::type early[EARLY ? TURNS : 1];
+
     const uint32_t mrow = (wave & 1) * (BM / 2) + lo, nrow = BM + (wave >> 1) * WB + lo;
     v4i x[2][MI], w[2][NI];
     auto read = [&](uint32_t step, int k, v4i(&xs)[MI], v4i(&ws)[NI]) {
@@ -152,6 +175,10 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
         if (ST - 1 < steps) load(ST - 1);
         read(0, 0, x[0], w[0]);
     }
+    if (EARLY && a.residual && left == 8 && !kg)
+#pragma unroll
+        for (uint32_t i = 0; i < TURNS; i++)
+            if (i * RI + lrow < rows_left) early[i] = *(const typename Vec8<O>::unaligned *)(res + (uint64_t)i * RI * a.ldr);
     for (uint32_t step = 0; step < steps; step++) {
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) {
@@ -202,14 +229,8 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
     // Results by rows: 32 of a wave's rows at a time go through LDS as 32-bit
     // floats, so that residuals are read and results written 16 bytes a lane
     // along the rows.  A lane's columns are the same in every row.
-    constexpr uint32_t LANES = WB / 8, RI = 64 / LANES;  // lanes of a row, rows of a turn
-    static_assert(64 % LANES == 0, "a lane keeps its columns");
     float *rows32 = (float *)lds + wave * 32 * PITCH;
-    const uint32_t mr = (wave & 1) * (BM / 2), lrow = lane / LANES, col = lane % LANES * 8, nc = (wave >> 1) * WB + col;
-    const int left = n0 + nc < a.n ? (int)min(8u, a.n - n0 - nc) : 0;
-    const uint32_t rows_left = left && m0 + mr < a.m ? (uint32_t)min((uint64_t)BM / 2, a.m - m0 - mr) : 0;
     O *y = (O *)a.y + (m0 + mr + lrow) * a.ldy + n0 + nc;
-    const O *res = (const O *)a.residual + (a.residual ? (m0 + mr + lrow) * a.ldr + n0 + nc : 0);
     float b[8], s[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 4) *(v4f *)(b + e) = *(const v4f *)(bias + nc + e), *(v4f *)(s + e) = *(const v4f *)(scale_w + nc + e);
@@ -239,7 +260,12 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
                 if (a.residual) {
                     if (left == 8) {
                         float g[8];
-                        load8(res, g);
+                        if (EARLY) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) g[e] = (float)early[EARLY ? m * (32 / RI) + i : 0][e];
+                        } else {
+                            load8(res, g);
+                        }
 #pragma unroll
                         for (int e = 0; e < 8; e++) f[e] += g[e];
                     } else {
@@ -260,7 +286,9 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
 // --------------------------------------------------------------- few rows --
 // Up to 16 * MF rows of x (one question, a few): w is read once, straight into
 // the matrix instructions' registers, 16 of its rows a workgroup; the waves
-// split k and join their sums in LDS.
+// split k and join their sums in LDS.  Bound by latency: a wave waits for four
+// steps' loads before it starts the next four (9 x 1536, k 384: 2.8 us; 8 x 4096, k 4096, 5.6:
+// 16.8 MB of w at 3.0 TB/s).
 constexpr uint32_t ROW_WAVES = 8;
 template <class O, int MF>
 __global__ __launch_bounds__(ROW_WAVES * 64) void linear_q8_rows(LinearQ8Args a) {
@@ -376,7 +404,8 @@ __global__ __launch_bounds__(256) void pack_codes(PackJob a, PackJob b, uint32_t
     }
 }
 
-// Rows up to which w goes straight to the registers.
+// Rows up to which w goes straight to the registers: 32 rows of 4096 x 4096 8.1 us,
+// 33 by tiles 8.7; of 768 x 768 3.4 and 5.3.
 constexpr uint64_t FEW_ROWS = 32;
 // A tile's loads have 32-bit offsets: 256 rows of as many codes reach 2^31
 // bytes.  Rows further apart are packed; k itself is far below.
@@ -464,34 +493,35 @@ hipError_t linear_q8_of(LinearQ8Args a, void *ws, hipStream_t s) {
     // 32768 x 4096, k 1024, bf16 192 -> 176 us, with GELU 251 -> 226.
     a.once = a.m * a.n * sizeof(O) > (64u << 20);
     // The shape that is done first: `fix` and rounds of the tiles that the card holds
-    // at a time, each a + b k and what its activations take; a last round of at most one tile a
-    // compute unit where two fit counts half (ns, fitted to 40..32768 x 384..4096 x
-    // 384..4096 without an activation, within 9%; the shapes chosen take 1.4% more
+    // at a time, each a + b k and what its activations take; where two fit a compute unit, a
+    // last round of at most one each is `part` hundredths of one (ns, fitted to 40..32768 x
+    // 384..4096 x 384..4096 without an activation: the shapes chosen take 0.1% more
     // than each size's best).  32768 x 1024, k 1024: 50.5 us in the last, the
-    // others 53.4, 59.2, 60.8, 75.4, 113 and 141; 2037 x 1024: 20.5, 14.9, 17.8, 14.0,
-    // 10.4, 8.7 and 10.4; 200 x 1024, k 4096: 51, 39, 43, 35, 26, 18 and 11.
+    // others 53.4, 59.2, 60.8, 75.4, 113, 107 and 141; 2037 x 768, k 768: 17.6, 12.6, 14.7,
+    // 11.8, 8.8, 7.5, 7.6 and 10.7; 200 x 1024, k 4096: 51, 39, 43, 35, 26, 18, 14 and 11.
     struct {
-        uint32_t bm, bn, cus, fix, a, b, gelu;  // cus: tiles of a compute unit
-    } const shapes[7] = {{64, 64, 1, 1307, 3029, 157, 470},    {64, 128, 1, 1055, 3385, 341, 940},
-                         {128, 128, 1, 808, 3379, 554, 1880},  {128, 256, 1, 0, 6374, 764, 3760},
-                         {192, 256, 1, 0, 9317, 947, 4400},    {128, 256, 2, 2381, 6954, 1661, 3000},
-                         {256, 256, 1, 0, 12627, 1132, 7500}};
+        uint32_t bm, bn, cus, part, fix, a, b, gelu;  // cus: tiles of a compute unit
+    } const shapes[8] = {{64, 64, 1, 100, 1501, 3029, 157, 470},    {64, 64, 2, 65, 2208, 2534, 376, 750},
+                         {64, 128, 1, 100, 1055, 3385, 341, 940},   {128, 128, 1, 100, 808, 3379, 494, 1880},
+                         {128, 256, 1, 100, 0, 6102, 764, 3760},    {192, 256, 1, 100, 0, 10542, 947, 4400},
+                         {128, 256, 2, 50, 2381, 6954, 1661, 3000}, {256, 256, 1, 100, 0, 12627, 1031, 7500}};
     int best = 0;
     uint64_t least = ~0ull;
-    for (int i = 0; i < 7; i++) {
+    for (int i = 0; i < 8; i++) {
         const auto &t = shapes[i];
         const uint64_t tiles = ((a.m + t.bm - 1) / t.bm) * ((a.n + t.bn - 1) / t.bn), at_a_time = 256 * t.cus, rest = tiles % at_a_time;
-        const uint64_t halves = tiles / at_a_time * 2 + (rest == 0 ? 0 : t.cus == 2 && rest <= 256 ? 1 : 2);
-        const uint64_t ns = t.fix + halves * (t.a + (uint64_t)t.b * a.k / 100 + (a.act > 1 ? t.gelu : 0)) / 2;
+        const uint64_t rounds = tiles / at_a_time * 100 + (rest == 0 ? 0 : t.cus == 2 && rest <= 256 ? t.part : 100);
+        const uint64_t ns = t.fix + rounds * (t.a + (uint64_t)t.b * a.k / 100 + (a.act > 1 ? t.gelu : 0)) / 100;
         if (ns < least) least = ns, best = i;
     }
     switch (best) {
     case 0: return tile_of<O, 64, 64, 2, 512, 2, 4>(a, s);
-    case 1: return tile_of<O, 64, 128, 2, 256, 2, 2>(a, s);
-    case 2: return tile_of<O, 128, 128, 4, 128, 4>(a, s);
-    case 3: return tile_of<O, 128, 256, 4, 128, 3>(a, s);
-    case 4: return tile_of<O, 192, 256, 4, 128, 2>(a, s);
-    case 5: return tile_of<O, 128, 256, 4, 64, 3>(a, s);
+    case 1: return tile_of<O, 64, 64, 2, 256, 2, 2>(a, s);
+    case 2: return tile_of<O, 64, 128, 2, 256, 2, 2>(a, s);
+    case 3: return tile_of<O, 128, 128, 4, 128, 4>(a, s);
+    case 4: return tile_of<O, 128, 256, 4, 128, 3>(a, s);
+    case 5: return tile_of<O, 192, 256, 4, 128, 2>(a, s);
+    case 6: return tile_of<O, 128, 256, 4, 64, 3>(a, s);
     default: return tile_of<O, 256, 256, 4, 128, 2>(a, s);
     }
 }
