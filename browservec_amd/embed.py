@@ -119,6 +119,12 @@ class EmbedOps:
             raise L.BVError(L.BV_E_UNSUPPORTED, f"{what}: {t.dtype} is not float32, float16 or bfloat16")
         return code
 
+    def _like(self, x, dtype):
+        """A contiguous tensor of x's shape."""
+        if x.is_contiguous():  # a third of the time of one from a shape
+            return self._empty_like(x, dtype=dtype)
+        return self._empty(x.shape, dtype=dtype, device=x.device)
+
     def _vector(self, t, n: int, what: str):
         if t.shape != (n,):
             _bad(f"{what} has shape {tuple(t.shape)}, not ({n},)")
@@ -312,7 +318,7 @@ class EmbedOps:
         if cu_q.shape != cu_k.shape or max_q < 0 or max_k < 0:
             _bad("attention: cu_q and cu_k differ in length, or max_q or max_k is negative")
         if out is None:
-            out = self._empty(sq, dtype=dtype, device=q.device)
+            out = self._like(q, dtype)
         elif out.shape != sq or out.dtype != dtype:
             _bad("attention: out differs from q in shape or type")
         else:
@@ -325,7 +331,10 @@ class EmbedOps:
         if window is None:
             a.window = 0
         else:
-            left, right = window
+            try:
+                left, right = window
+            except (TypeError, ValueError):
+                _bad(f"attention: window {window!r} is not (left, right)")
             a.window, a.window_left, a.window_right, a.sinks = 1, _keys(left), _keys(right), _keys(sinks)
         if scale is not None and a.scale == 0:  # in 32 bits; the library's word for its default
             _bad(f"attention: scale {scale} is 0 in 32 bits")
@@ -376,12 +385,6 @@ class EmbedOps:
         elif out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
             _bad("norm: out differs from x in shape, or in type from out_dtype")
         return self._normed("norm", x, weight, bias, kind, eps, 0, False, None, out)
-
-    def _like(self, x, dtype):
-        """A contiguous tensor of x's shape."""
-        if x.is_contiguous():  # a third of the time of one from a shape
-            return self._empty_like(x, dtype=dtype)
-        return self._empty(x.shape, dtype=dtype, device=x.device)
 
     def _add_norm(self, what: str, x, residual, weight, bias, kind, eps, total, out, scales):
         a, address = self._add

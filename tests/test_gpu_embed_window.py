@@ -210,7 +210,7 @@ def test_window_refusals_and_the_struct_before_it(ops):  # noqa: F811
 
     say("window refusals")
     q, cu = rand((8, 2, 64), 1, BF).cuda(), dev_cu([0, 8])
-    for kw in (dict(window=(-1, 0)), dict(window=(0, -2)), dict(window=(0, 0), sinks=-1)):
+    for kw in (dict(window=(-1, 0)), dict(window=(0, -2)), dict(window=(0, 0), sinks=-1), dict(window=5), dict(window=(1, 2, 3))):
         with pytest.raises(L.BVError) as e:
             ops.attention(q, q, q, cu, **kw)
         assert e.value.code == L.BV_E_INVALID and str(e.value)
@@ -274,3 +274,20 @@ def test_window_of_many_texts(ops):  # noqa: F811
         for causal, left, right, sinks in ((False, 16, 30, 0), (True, 50, 0, 2)):
             o = ops.attention(q, k, v, dev_cu(cu), causal=causal, window=(left, right), sinks=sinks, max_q=300)
             inside(o, *window_want(q, k, v, cu, cu, causal, left, right, sinks), "many texts")
+
+
+def test_short_window_of_far_keys_and_odd_rows(ops):  # noqa: F811
+    """Keys past 2^31 elements; queries and results at odd addresses; no keys at all."""
+    say("short window, far keys")
+    nk, hk, d, tail = 2 ** 31 // 1024 + 700, 4, 256, 300
+    big = torch.zeros(nk, hk, d, dtype=BF, device="cuda")
+    big[-tail:] = rand((tail, hk, d), 1, BF).cuda()
+    k, v = big[:, :, :128], big[:, :, 128:]
+    q = rand((200, hk, 129), 5, BF).cuda()[:, :, 1:]
+    out = torch.full((200, hk, 131), 7.0, dtype=BF, device="cuda")
+    o = ops.attention(q, k, v, dev_cu([0, 200]), dev_cu([0, nk]), max_q=200, window=(40, 0), out=out[:, :, 1:129])
+    near = [t[-250:].contiguous() for t in (k, v)]
+    inside(o, *window_want(q, *near, [0, 200], [0, 250], True, 40, 0, 0), "far keys")
+    assert torch.all(out[:, :, 0] == 7) and torch.all(out[:, :, 129:] == 7)
+    o = ops.attention(q[:, :, :64], k[:0, :, :64], v[:0, :, :64], dev_cu([0, 200]), dev_cu([0, 0]), causal=False, window=(40, 40), sinks=3)
+    assert torch.all(o == 0)
