@@ -55,7 +55,7 @@ __device__ __forceinline__ void activate8(float (&f)[8], int act) {
 
 // The end of eight neighbouring results of a row, columns n on: residual,
 // rounding, store.
-template <class O, bool ONCE = false, class Args>
+template <class O, class Args>
 __device__ __forceinline__ void finish8(const Args &a, uint64_t m, uint32_t n, float (&f)[8]) {
     const int left = (int)min(8u, a.n - n);
     if (a.residual) {
@@ -70,7 +70,7 @@ __device__ __forceinline__ void finish8(const Args &a, uint64_t m, uint32_t n, f
             for (int i = 0; i < 8; i++) f[i] += (float)r[min(i, left - 1)];
         }
     }
-    store8<ONCE>((O *)a.y + m * a.ldy + n, left, f);
+    store8((O *)a.y + m * a.ldy + n, left, f);
 }
 
 }  // namespace

@@ -77,6 +77,19 @@ def test_linear_q8_many_tiles(ops, m, n, k, out):  # noqa: F811
     inside(y, *linear_q8_want(x, sx, w, sw, b, r, "silu", out), "linear_q8")
 
 
+@pytest.mark.parametrize("out", [BF, F32])
+@pytest.mark.parametrize("m,n,k", [(16400, 1000, 1003), (4112, 4096, 1003), (20011, 1024, 4096)])
+def test_linear_q8_rows_behind_whole_rounds(ops, m, n, k, out):  # noqa: F811
+    """Sizes whose last rows go in other tiles than the rest; the result lies in wider rows."""
+    say("linear_q8 rows behind", m, n, k, out)
+    x, w, sx, sw = codes((m, k), 1).cuda(), codes((n, k), 2).cuda(), scales(m, 3).cuda(), scales(n, 4).cuda()
+    b, r = rand((n,), 5, F32).cuda(), rand((m, n + 8), 6, out).cuda()[:, :n]
+    y = torch.full((m + 1, n + 8), 7.0, dtype=out, device="cuda")
+    ops.linear_q8(x, sx, w, sw, bias=b, residual=r, activation="gelu", out_dtype=out, out=y[:m, :n])
+    inside(y[:m, :n], *linear_q8_want(x, sx, w, sw, b, r, "gelu", out), "linear_q8")
+    assert (y[m:] == 7).all() and (y[:, n:] == 7).all()
+
+
 @pytest.mark.parametrize("m", [3, 40, 600])
 def test_linear_q8_of_the_largest_sums(ops, m):  # noqa: F811
     """The longest k of products of -128 and -128: sums of 2^31 - 2^14."""
