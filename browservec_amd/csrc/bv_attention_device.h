@@ -388,7 +388,7 @@ __device__ __forceinline__ void store_by_rows(const AttentionArgs &a, const Plac
 // 573 to 612 us by card, 840 to 900 TFLOP/s of visible pairs; 6% more are computed, in tiles
 // that the window cuts and the first keys' own.
 template <class T, int D, int KT, int GROUPS, bool DIRECT, bool LOCAL>
-__global__ __launch_bounds__(256 * GROUPS, D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
+__global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {
     typedef typename Vec8<T>::type V;
     constexpr int THREADS = 256 * GROUPS, CH = D / 8, CHUNKS = KT * CH, NL = (CHUNKS + THREADS - 1) / THREADS;

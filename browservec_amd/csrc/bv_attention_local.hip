@@ -19,6 +19,13 @@ namespace {
 // there are two, 71; weights made tile by tile, which saves registers, 63.
 // FIRSTS: the sequence's first 32 keys, of which `sinks` count, are a tile of their
 // own; a key of the window counts there alone.
+//   They lie in LDS before the window's, no more than count and fill a wave's load
+// (whole rows of 1024 bytes): their tile's other rows are the window's, and get no weight.
+template <int D>
+constexpr uint32_t whole_rows(uint32_t n) {
+    constexpr uint32_t of = D == 128 ? 4 : D == 64 ? 8 : 16;
+    return (n + of - 1) / of * of;
+}
 template <class T, int D, int NT, bool FIRSTS>
 __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_window(AttentionArgs a, AttentionPlan pl, uint64_t first,
                                                                           uint32_t slots, uint32_t lds_rows) {
@@ -52,21 +59,21 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
         q[i] = raw8((const T *)a.q + token * a.sq + head * a.sqh, i * 16 + hi * 8, a.d, in, zeros);
         if (pl.negate) q[i] = -q[i];
     }
-    // LDS row r is key from.lo + r; the first keys follow at lds_rows - 32.  Rows past
-    // the last key repeat it: they get no weight, and a value that is not finite is
+    // LDS row first_rows + r is key from.lo + r.  Rows past the last key repeat it: they get no weight, and a value that is not finite is
     // found in the results.
     const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
     const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
-    const int32_t window_rows = (int32_t)lds_rows - (FIRSTS ? 32 : 0);
-    const int32_t rows = min(window_rows, (to.hi - from.lo + 31 + 31) & ~31);  // loaded: what the waves' tiles reach
+    const int32_t first_rows = FIRSTS ? whole_rows<D>(a.sinks) : 0;
+    const int32_t rows = min((int32_t)lds_rows - first_rows, (to.hi - from.lo + 31 + 31) & ~31);  // loaded: what the waves' tiles reach
     // Where rows have 4, 8 or 16 chunks a thread's chunks lie at the same place of
     // every PASS-th row, whose swizzle is the same.
     constexpr int PASS = 256 / CH;
     constexpr bool REGULAR = 256 % CH == 0;
-    auto load_rows = [&](const char *base, uint64_t step, bool values, int32_t k0, int32_t rows, uint32_t to) {
+    auto load_rows = [&](const char *base, uint64_t step, bool values, int32_t k0, int32_t rows, uint32_t row0) {
         const int32_t chunks = rows * CH;
-        const uint32_t r0 = tid / CH, c0 = ((tid % CH) ^ (values ? value_swizzle<D>(r0) : key_swizzle<D>(r0))) * 8;
+        const uint32_t to = row0 * D * 2, r0 = tid / CH;
+        const uint32_t c0 = ((tid % CH) ^ (values ? value_swizzle<D>(row0 + r0) : key_swizzle<D>(row0 + r0))) * 8;
         const uint32_t off = (r0 * (uint32_t)step + c0) * 2;
         const char *at = base + (uint64_t)k0 * step * 2;
         for (int32_t i = 0; i < chunks; i += 256) {
@@ -76,7 +83,7 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
                 if (c0 < a.d) lds_load16(at, off, into);
             } else {
                 const uint32_t idx = i + tid, r = idx / CH;
-                const uint32_t c = REGULAR ? c0 : ((idx % CH) ^ (values ? value_swizzle<D>(r) : key_swizzle<D>(r))) * 8;
+                const uint32_t c = REGULAR ? c0 : ((idx % CH) ^ (values ? value_swizzle<D>(row0 + r) : key_swizzle<D>(row0 + r))) * 8;
                 const uint64_t key = (uint32_t)min(REGULAR ? k0 + (int32_t)r0 : k0 + (int32_t)r, p.lk - 1);
                 if (c < a.d) lds_dma16(base + (key * step + c) * 2, into);
             }
@@ -87,8 +94,8 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
         }
     };
     auto load = [&](const char *base, uint64_t step, bool values) {
-        if (to.hi > from.lo) load_rows(base, step, values, from.lo, rows, 0);
-        if (FIRSTS && to.first > 0) load_rows(base, step, values, 0, 32, window_rows * D * 2);
+        if (to.hi > from.lo || (FIRSTS && to.first > 0)) load_rows(base, step, values, from.lo, rows, first_rows);
+        if (FIRSTS && to.first > 0) load_rows(base, step, values, 0, first_rows, 0);
     };
     if (a.d < D) {  // what lies past d
         for (uint32_t i = tid; i < lds_rows * CH; i += 256) *(v4i *)(lds + i * 16) = v4i{0, 0, 0, 0};
@@ -105,7 +112,7 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
     V f[FR];
     const bool firsts = FIRSTS && wto.first > 0;
     auto any = [&](int t) { return t < NT ? t < nt : firsts; };
-    auto lds_row = [&](int t) { return (uint32_t)(t < NT ? w0 + t * 32 : window_rows); };
+    auto lds_row = [&](int t) { return (uint32_t)(t < NT ? first_rows + w0 + t * 32 : 0); };
     auto read_keys = [&](int t, V(&f)[FR]) {
         const uint32_t r = lds_row(t) + lo;
         const uint32_t at = r * D * 2, sw = key_swizzle<D>(r);
@@ -224,9 +231,12 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
 // both sides, 16 heads over 4, 8 x 2000..4096 tokens: d = 64 79 us against 76, with 4
 // first keys 87 against 85; d = 32 45 against 50 but with first keys 63 against 60; d = 96 101
 // against 141, d = 128 120 against 179).
-int window_tiles(const AttentionArgs &a) {
+uint64_t keys_of_wave(const AttentionArgs &a) {
     const uint64_t group = a.hq / a.hk;
-    const uint64_t keys = (31 + group - 1) / group + (uint64_t)a.left + (a.causal ? 0 : a.right) + 1;
+    return (31 + group - 1) / group + (uint64_t)a.left + (a.causal ? 0 : a.right) + 1;
+}
+int window_tiles(const AttentionArgs &a) {
+    const uint64_t keys = keys_of_wave(a);
     if (a.sinks > 32 || keys > 288) return 0;
     return keys <= 160 ? 5 : a.d > 64 || (a.d <= 32 && !a.sinks) ? 9 : 0;
 }
@@ -240,9 +250,12 @@ template <class T, int D, int NT, bool FIRSTS>
 hipError_t window_of(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
     const uint32_t group = a.hq / a.hk;
     const uint64_t slots = a.tq * group / 128 + a.batch;
-    // the waves' first rows lie at most 96 rows apart, each reads NT tiles on; the
-    // first keys' place, a multiple of 32, has the same swizzle as its rows
-    const uint32_t span = (96 + group - 1) / group + NT * 32, rows = FIRSTS ? (span + 31) / 32 * 32 + 32 : span;
+    // The waves' first rows lie at most 96 rows apart, and each reads the tiles that its
+    // keys reach, not NT: as little LDS as a call needs (d = 128, 16 heads over 4, the last 201
+    // keys and 4 first ones, 8 x 2000..4096 tokens: two workgroups a CU, 123 us, one 194).  The
+    // results take 128 rows.
+    const uint32_t span = (96 + group - 1) / group + (uint32_t)(keys_of_wave(a) + 31) / 32 * 32;
+    const uint32_t rows = std::max(128u, whole_rows<D>(span) + (FIRSTS ? whole_rows<D>(a.sinks) : 0));
     const uint32_t bytes = rows * D * 2;
     const uint64_t most = std::max<uint64_t>(1, (1u << 22) / a.hk);  // launches of fewer than 2^32 threads
     for (uint64_t f = 0; f < slots; f += most) {

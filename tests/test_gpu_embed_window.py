@@ -291,3 +291,43 @@ def test_short_window_of_far_keys_and_odd_rows(ops):  # noqa: F811
     assert torch.all(out[:, :, 0] == 7) and torch.all(out[:, :, 129:] == 7)
     o = ops.attention(q[:, :, :64], k[:0, :, :64], v[:0, :, :64], dev_cu([0, 200]), dev_cu([0, 0]), causal=False, window=(40, 40), sinks=3)
     assert torch.all(o == 0)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 1, 128), (2, 2, 128), (8, 2, 64), (4, 1, 96), (6, 2, 32), (2, 1, 104)])
+def test_short_windows_and_their_first_keys(ops, hq, hk, d):  # noqa: F811
+    """First keys of every number beside windows of few and many keys, queries before
+    the first key, whose window is empty, among them."""
+    say("first keys", hq, hk, d)
+    nq, nk = [333, 200, 1, 70, 150], [333, 90, 1, 260, 1]
+    cq, ck = cu_of(nq), cu_of(nk)
+    q, k, v = rand((cq[-1], hq, d), 1, BF, 1.5).cuda(), rand((ck[-1], hk, d), 2, BF).cuda(), rand((ck[-1], hk, d), 3, BF).cuda()
+    for left, right, sinks in [(0, 0, 1), (5, 3, 4), (150, 0, 4), (120, 0, 5), (200, 0, 8), (250, 0, 9), (100, 100, 16), (60, 70, 17),
+                               (31, 31, 31), (200, 50, 32), (250, 0, 3), (0, 0, 32)]:
+        for causal in (False, True):
+            o = ops.attention(q, k, v, dev_cu(cq), dev_cu(ck), causal=causal, window=(left, right), sinks=sinks)
+            inside(o, *window_want(q, k, v, cq, ck, causal, left, right, sinks), f"first keys {left} {right} {sinks} {causal}")
+
+
+def test_a_windows_values_that_are_not_finite_reach_whoever_sees_them(ops):  # noqa: F811
+    """An infinite and a NaN value within some rows' windows: those rows are as the
+    formula has them, the others as with finite values."""
+    n, d = 1500, 64
+    for hq, hk, left, sinks in ((4, 2, 40, 0), (4, 2, 700, 3), (2, 2, 300, 0)):
+        say("not finite", hq, hk, left, sinks)
+        q, k, v = rand((n, hq, d), 1, BF).cuda(), rand((n, hk, d), 2, BF).cuda(), rand((n, hk, d), 3, BF).cuda()
+        bad = v.clone()
+        bad[500, 0, 3], bad[901, hk - 1, 60] = float("inf"), float("nan")
+        run = lambda v: ops.attention(q, k, v, dev_cu([0, n]), window=(left, 0), sinks=sinks).cpu()  # noqa: E731
+        good, got = run(v), run(bad)
+        want, bound = window_want(q, k, v, [0, n], [0, n], True, left, 0, sinks)
+        sees = seen_of(n, n, True, left, 0, sinks)
+        hit = torch.zeros(n, hq, d, dtype=torch.bool)
+        group = hq // hk
+        for key, head, at, value in ((500, 0, 3, float("inf")), (901, hk - 1, 60, float("nan"))):
+            rows = sees[:, key]
+            for h in range(head * group, (head + 1) * group):
+                hit[rows, h, at] = True
+                x = got[rows, h, at].float()
+                assert (x == value).all() if value == value else x.isnan().all()
+        assert torch.isfinite(got[~hit].float()).all() and torch.isfinite(good.float()).all()
+        assert ((got.double() - want).abs() <= bound)[~hit].all()
