@@ -381,12 +381,14 @@ __device__ __forceinline__ void store_by_rows(const AttentionArgs &a, const Plac
 // without a mask) they are busy for 12 and 38%: what is left is the chain at a
 // workgroup's start, offsets, queries and first keys one after the other.
 //   Registers spilled by a lane: with turns 3 at D = 128 and 23 at D = 256 (with a
-// window 17 and 28, outside the loop's common path).  4 x 4096 tokens, 8 heads, no
+// window 3 and 22, outside the loop's common path).  4 x 4096 tokens, 8 heads, no
 // mask: d = 128 344 us, at odd addresses 791; d = 104 330, d = 100, whose elements are
 // loaded one by one, 1453; d = 256 1229, at odd addresses 2714.
 //   A window: 32768 tokens, 8 heads of 128 over 2, the last 4096 keys and 4 first ones, f16,
-// 573 to 612 us by card, 840 to 900 TFLOP/s of visible pairs; 6% more are computed, in tiles
-// that the window cuts and the first keys' own.
+// 565 to 591 us by card, 870 to 910 TFLOP/s of visible pairs; 6% more are computed, in tiles
+// that the window cuts and the first keys' own.  4 x 4001..8192 tokens, 16 heads over 4, the last
+// 512 keys: d = 64 90 to 103 us, of which half does not grow with the window (1024 keys
+// 150); d = 32 70, with four workgroups a CU (one register spilled), 77 with three.
 template <class T, int D, int KT, int GROUPS, bool DIRECT, bool LOCAL>
 __global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {

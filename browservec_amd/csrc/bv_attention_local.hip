@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
 
 // A wave's tiles of a window's keys, or 0 for attention_tile: the window, or the first
 // keys, are too many, or nine tiles' scores leave a SIMD too few waves (128 on
-// both sides, 16 heads over 4, 8 x 2000..4096 tokens: d = 64 79 us against 76, with 4
+// both sides, 16 heads over 4, 8 x 2000..4096 tokens: d = 64 79 us against 69, with 4
 // first keys 87 against 85; d = 32 45 against 50 but with first keys 63 against 60; d = 96 101
 // against 141, d = 128 120 against 179).
 uint64_t keys_of_wave(const AttentionArgs &a) {
