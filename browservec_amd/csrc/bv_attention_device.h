@@ -96,7 +96,7 @@ template <int KT>
 struct Tiles {
     int32_t firsts, b0, tiles;
     __device__ __forceinline__ Tiles(const View &from, const View &to) {
-        firsts = (to.first + KT - 1) / KT;
+        firsts = (int32_t)(((uint32_t)to.first + KT - 1) / KT);
         b0 = from.lo;
         int32_t end = to.hi;
         if (firsts && (int64_t)firsts * KT >= b0) firsts = 0, b0 = 0, end = max(end, to.first);
@@ -113,7 +113,7 @@ struct Seen {
     __device__ __forceinline__ Seen(const Tiles<KT> &tiles, const View &from, const View &to) {
         auto down = [&](int32_t key) { return tiles.firsts + max(0, key - tiles.b0) / KT; };
         auto up = [&](int32_t key) { return tiles.firsts + (int32_t)(((uint32_t)max(0, key - tiles.b0) + KT - 1) / KT); };
-        firsts = (to.first + KT - 1) / KT, all_firsts = from.first / KT;
+        firsts = (int32_t)(((uint32_t)to.first + KT - 1) / KT), all_firsts = from.first / KT;
         begin = down(from.lo), end = up(to.hi), all_begin = up(to.lo), all_end = down(from.hi);
     }
     __device__ __forceinline__ bool any(int32_t t) const { return t < firsts || (t >= begin && t < end); }
@@ -677,7 +677,9 @@ __global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 :
         if (!g) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
-    if (LOCAL) {  // a value that is not finite has made the sums of all of its tile's rows so (the tiles' looked through: 5% at D = 64)
+    // LOCAL: a value that is not finite has made the sums of all rows of its tile so
+    // (looking through the tiles' values took 5% longer at D = 64).
+    if (LOCAL) {
         float nought = 0;
 #pragma unroll
         for (int d = 0; d < DB; d++)
@@ -728,7 +730,8 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
     const int32_t t1 = part_of<KT>(pl, split, tiles.tiles, t0);
     const Seen<KT> seen(tiles, from, to);
     const int32_t first_query = (uint32_t)p.row0 / group;
-    const int32_t behind = (int32_t)((uint32_t)row / group) - first_query - (int32_t)hi * 4, most = (int32_t)(((uint32_t)p.row0 + 31) / group) - first_query;
+    const int32_t behind = (int32_t)((uint32_t)row / group) - first_query - (int32_t)hi * 4;
+    const int32_t most = (int32_t)(((uint32_t)p.row0 + 31) / group) - first_query;
     const bool in = row < p.rows;
     const int32_t query = in ? (uint32_t)row / group : 0;
     const int64_t token = p.qb + query, head = hk * group + (in ? row - query * (int32_t)group : 0);

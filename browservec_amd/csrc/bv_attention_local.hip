@@ -17,10 +17,10 @@ namespace {
 // us, 3.8 TB/s of 5.1 that a copy reaches (vector unit busy for 42% of the cycles, matrix
 // cores for 11; attention_tile 79).  Four workgroups a CU: with keys and values in LDS side by side
 // there are two, 71; weights made tile by tile, which saves registers, 63.
-// FIRSTS: the sequence's first 32 keys, of which `sinks` count, are a tile of their
-// own; a key of the window counts there alone.
-//   They lie in LDS before the window's, no more than count and fill a wave's load
-// (whole rows of 1024 bytes): their tile's other rows are the window's, and get no weight.
+// FIRSTS: the sequence's first keys are a tile of their own, in which keys of the window
+// do not count.  They lie in LDS before the window's, as many rows as `sinks` and a
+// wave's whole loads of 1024 bytes take; the tile's other rows are the window's, without
+// weight.
 template <int D>
 constexpr uint32_t whole_rows(uint32_t n) {
     constexpr uint32_t of = D == 128 ? 4 : D == 64 ? 8 : 16;
@@ -59,8 +59,8 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
         q[i] = raw8((const T *)a.q + token * a.sq + head * a.sqh, i * 16 + hi * 8, a.d, in, zeros);
         if (pl.negate) q[i] = -q[i];
     }
-    // LDS row first_rows + r is key from.lo + r.  Rows past the last key repeat it: they get no weight, and a value that is not finite is
-    // found in the results.
+    // LDS row first_rows + r is key from.lo + r.  Rows past the last key repeat it: they
+    // get no weight, and a value that is not finite is found in the results.
     const char *kp = (const char *)((const T *)a.k + p.kb * a.sk + hk * a.skh);
     const char *vp = (const char *)((const T *)a.v + p.kb * a.sv + hk * a.svh);
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
@@ -226,15 +226,16 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
     store_by_rows<T, D>(a, p, group, hk, o, sum, wrow, view.any(), lds + wave * 32 * D * 2);
 }
 
-// A wave's tiles of a window's keys, or 0 for attention_tile: the window, or the first
-// keys, are too many, or nine tiles' scores leave a SIMD too few waves (128 on
-// both sides, 16 heads over 4, 8 x 2000..4096 tokens: d = 64 79 us against 69, with 4
-// first keys 87 against 85; d = 32 45 against 50 but with first keys 63 against 60; d = 96 101
-// against 141, d = 128 120 against 179).
+// The keys that a wave's 32 rows see in a window.
 uint64_t keys_of_wave(const AttentionArgs &a) {
     const uint64_t group = a.hq / a.hk;
     return (31 + group - 1) / group + (uint64_t)a.left + (a.causal ? 0 : a.right) + 1;
 }
+// A wave's tiles of a window's keys, or 0 for attention_tile: the window, or the first
+// keys, are too many, or nine tiles' scores leave a SIMD too few waves (128 on
+// both sides, 16 heads over 4, 8 x 2000..4096 tokens: d = 64 79 us against 69, with 4
+// first keys 87 against 85; d = 32 45 against 50 but with first keys 63 against 60; d = 96 101
+// against 137, d = 128 119 against 157).
 int window_tiles(const AttentionArgs &a) {
     const uint64_t keys = keys_of_wave(a);
     if (a.sinks > 32 || keys > 288) return 0;
