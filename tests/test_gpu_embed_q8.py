@@ -429,11 +429,11 @@ def test_c_refusals(ops):  # noqa: F811
             setattr(a, k, v)
         return fn(ops.handle, ctypes.addressof(a))
 
-    base = dict(out_dtype=2, activation=0, m=4, n=8, k=16, x=p, w=p + 1024, x_scales=p + 2048, w_scales=p + 3072, y=p + 4096)
+    base = dict(out_dtype=2, activation=0, m=4, n=8, k=16, x=p, w=p + 1024, x_scales=p + 2048, w_scales=p + 2560, y=p + 4096)
     assert call(L.LinearQ8Args, lib.bv_embed_linear_q8, base, {}) == L.BV_OK
     for kw in (dict(size=8), dict(x=None), dict(w=None), dict(x_scales=None), dict(w_scales=None), dict(y=None), dict(x_stride=15),
                dict(y_stride=7), dict(out_dtype=3), dict(bias=p + 8192, bias_dtype=3), dict(activation=9), dict(x_scales=p + 2049),
-               dict(y=p), dict(y=p + 2048), dict(y=p + 3102), dict(m=2 ** 62), dict(residual=p + 4098), dict(bias=p + 4096), dict(k=131072)):
+               dict(y=p), dict(y=p + 2048), dict(y=p + 2590), dict(m=2 ** 62), dict(residual=p + 4098), dict(bias=p + 4096), dict(k=131072)):
         assert call(L.LinearQ8Args, lib.bv_embed_linear_q8, base, kw) in (L.BV_E_INVALID, L.BV_E_UNSUPPORTED), kw
         assert lib.bv_last_error()
     base = dict(dtype=2, residual_dtype=2, out_dtype=3, norm=2, dim=16, eps=1e-5, tokens=4, x=p, residual=p + 1024, total=p + 2048,
