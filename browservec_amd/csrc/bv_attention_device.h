@@ -125,6 +125,14 @@ __device__ __forceinline__ View rows_view(const AttentionArgs &a, const Place &p
     return LOCAL ? view_of(a, p, query) : View{0, seen_by(a, p, query), 0};
 }
 
+// Tiles of all rows up to `to`.  Without a window they begin at key 0, and this is all
+// that is wanted of them (by way of Tiles, whose counts have 64 bits, 4 x 4096 tokens, 8
+// heads of 256 took 1336 us; 1296 so).
+template <bool LOCAL, int KT>
+__device__ __forceinline__ int32_t tile_count(const Tiles<KT> &tiles, const View &to) {
+    return LOCAL ? tiles.tiles : (to.hi + KT - 1) / KT;
+}
+
 // -inf for the keys of a tile that the lane's row does not see.  query: the wave's first;
 // rows: how many queries the lane's row is behind it, less four for lanes of the upper
 // half; most: the wave's last query's.  Ends that the wave shares are worked out once
@@ -411,7 +419,7 @@ __global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 :
     const View from = rows_view<LOCAL>(a, p, (uint32_t)p.row0 / group), to = rows_view<LOCAL>(a, p, (uint32_t)(row_end - 1) / group);
     const Tiles<KT> tiles(from, to);
     int32_t t0;
-    const int32_t t1 = part_of<KT>(pl, split, tiles.tiles, t0);
+    const int32_t t1 = part_of<KT>(pl, split, tile_count<LOCAL, KT>(tiles, to), t0);
 
     // this wave's rows, and the tiles that some of them see
     const int32_t wrow = p.row0 + wave * 32, wend = min(p.rows, wrow + 32);
@@ -450,7 +458,11 @@ __global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 :
     auto load = [&](int32_t t, uint32_t to, bool values) {
         const uint64_t step = values ? a.sv : a.sk;
         const int32_t k0 = LOCAL ? tiles.key(t) : t * KT;
-        const char *base = (values ? vp : kp) + (uint64_t)k0 * step * 2;
+        // t * KT in 64 bits steps along with t; in 32 and then widened it is a product of
+        // its own for every tile (4 x 4096 tokens, 8 heads of 64: 193 us, stepping 188).
+        // Rows that go through registers leave none to step with (heads of 100: 2230,
+        // as a product 1470).
+        const char *base = (values ? vp : kp) + (DIRECT && !LOCAL ? (uint64_t)t * KT : (uint64_t)k0) * step * 2;
         if (DIRECT && REGULAR && k0 + KT <= p.lk) {
             if ((values ? vc : kc) < a.d)
 #pragma unroll
@@ -727,7 +739,7 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
     const View from = rows_view<LOCAL>(a, p, (uint32_t)p.row0 / group), to = rows_view<LOCAL>(a, p, (uint32_t)(wend - 1) / group);
     const Tiles<KT> tiles(from, to);
     int32_t t0;
-    const int32_t t1 = part_of<KT>(pl, split, tiles.tiles, t0);
+    const int32_t t1 = part_of<KT>(pl, split, tile_count<LOCAL, KT>(tiles, to), t0);
     const Seen<KT> seen(tiles, from, to);
     const int32_t first_query = (uint32_t)p.row0 / group;
     const int32_t behind = (int32_t)((uint32_t)row / group) - first_query - (int32_t)hi * 4;
@@ -748,7 +760,8 @@ __global__ __launch_bounds__(256, 1) void attention_few(AttentionArgs a, Attenti
     auto load = [&](int32_t t) {
         const uint32_t to = lds0 + (uint32_t)(t - t0) % ST * 2 * TILE;
         const int32_t k0 = LOCAL ? tiles.key(t) : t * KT;
-        const char *kb = kp + (uint64_t)k0 * a.sk * 2, *vb = vp + (uint64_t)k0 * a.sv * 2;
+        const uint64_t key = LOCAL ? (uint64_t)k0 : (uint64_t)t * KT;  // as in attention_tile
+        const char *kb = kp + key * a.sk * 2, *vb = vp + key * a.sv * 2;
         const uint32_t last = p.lk - 1 - k0;
 #pragma unroll
         for (int i = 0; i < NL; i++) {
