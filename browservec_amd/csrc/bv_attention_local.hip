@@ -210,13 +210,20 @@ __global__ __launch_bounds__(256, NT <= 5 && D <= 64 ? 4 : 2) void attention_win
         __builtin_amdgcn_sched_barrier(0);
     }
     // A value that is not finite reaches rows that do not see it as 0 * inf: where a
-    // result is not finite, the rows are done one by one.
+    // result is not finite, the rows are done one by one, but for those whose weights
+    // have no finite sum (as in attention_tile).
     float check = 0;
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) check = fmaf(o[d][e], 0.0f, check);
-    if (__syncthreads_or(!(check == 0.0f))) {
+    const bool not_finite = in && !(check == 0.0f);
+    bool alone = __syncthreads_or(not_finite);
+    if (alone) {
+        const float total = halves_sum(sum);
+        alone = __syncthreads_or(not_finite && total == total);
+    }
+    if (alone) {
         float *own = (float *)lds + wave * 320;
         const Tiles<32> tiles(from, to);
         for (int32_t i = wrow; i < wend; i++)
