@@ -300,7 +300,8 @@ class EmbedOps:
         that at it and `right` after it (None: all on that side), and the
         sequence's first `sinks` keys; query i's place is i + keys - queries of
         its sequence.  causal hides what comes after a query's place, of the
-        first keys too."""
+        first keys too.  Keys that no query sees may hold anything, but stay
+        readable: some are loaded beside those that are seen."""
         a, address = self._attention
         if cu_k is None:
             cu_k = cu_q

@@ -509,8 +509,11 @@ int bv_embed_rotary_table(const bv_embed_rotary_scaling *scaling, uint32_t table
  * (BV_ALL_KEYS or any number from 2^31 - 1 on: no end on that side).  The place of
  * query i of lq is i + lk - lq among lk keys: the last query's is the last key.
  * causal still hides all keys after a query's place, of the first keys too.  Keys
- * that no query sees are not read.  Callers whose struct ends before `window` (size
- * BV_EMBED_ATTENTION_ARGS_V1) have none. */
+ * that no query sees change nothing and most of them are not read, but all have to
+ * be readable memory: keys are loaded in tiles of up to 128, which reach past the
+ * window and past the first keys, and where those tiles would meet, all between the two.
+ * Callers whose struct ends before `window` (size BV_EMBED_ATTENTION_ARGS_V1) have
+ * none. */
 #define BV_ALL_KEYS 0xffffffffu
 #define BV_EMBED_ATTENTION_ARGS_V1 168
 typedef struct bv_embed_attention_args {
