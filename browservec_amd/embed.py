@@ -300,8 +300,9 @@ class EmbedOps:
         that at it and `right` after it (None: all on that side), and the
         sequence's first `sinks` keys; query i's place is i + keys - queries of
         its sequence.  causal hides what comes after a query's place, of the
-        first keys too.  Keys that no query sees may hold anything, but stay
-        readable: some are loaded beside those that are seen."""
+        first keys too.  Without a window all are seen, whatever `sinks`.  Keys that
+        no query sees may hold anything, but stay readable: some are loaded beside
+        those that are seen."""
         a, address = self._attention
         if cu_k is None:
             cu_k = cu_q
@@ -331,6 +332,8 @@ class EmbedOps:
         a.max_q, a.max_k, a.scale = min(max_q, sq[0]), min(max_k, sk[0]), 0.0 if scale is None else scale
         if window is None:
             a.window = 0
+            if sinks:
+                _keys(sinks)  # its checks alone: all keys are seen
         else:
             try:
                 left, right = window
