@@ -272,12 +272,16 @@ hipError_t window_of(const AttentionArgs &a, const AttentionPlan &pl, hipStream_
     }
     return hipGetLastError();
 }
+// window_tiles says 9 for D > 64, and for D = 32 where there are no first keys.
 template <class T, int D>
 hipError_t window_sized(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
-    if (window_tiles(a) == 5) return a.sinks ? window_of<T, D, 5, true>(a, pl, s) : window_of<T, D, 5, false>(a, pl, s);
-    if constexpr (D == 64) return hipErrorInvalidValue;  // window_tiles does not say 9
-    else if constexpr (D == 32) return window_of<T, D, 9, false>(a, pl, s);
-    else return a.sinks ? window_of<T, D, 9, true>(a, pl, s) : window_of<T, D, 9, false>(a, pl, s);
+    if constexpr (D != 64)
+        if (window_tiles(a) == 9) {
+            if constexpr (D > 64)
+                if (a.sinks) return window_of<T, D, 9, true>(a, pl, s);
+            return window_of<T, D, 9, false>(a, pl, s);
+        }
+    return a.sinks ? window_of<T, D, 5, true>(a, pl, s) : window_of<T, D, 5, false>(a, pl, s);
 }
 template <class T>
 hipError_t window_typed(const AttentionArgs &a, const AttentionPlan &pl, hipStream_t s) {
