@@ -24,7 +24,7 @@ SOURCES = (["bv_kernels.hip"] + [f"bv_scan_{c}.hip" for c in SCAN_CODECS] +
            ["bv_ivf.hip", "bv_mq.hip", "bv_mqf.hip", "bv_pick.hip", "bv_select.hip", "bv_graph.hip", "bv_linear.hip",
             "bv_linear_q8.hip", "bv_attention.hip", "bv_attention_local.hip", "bv_rows.hip", "bv_add_norm.hip", "bv_embed.cpp", "bv_api.cpp"])
 HEADERS = ["bv_kernels.h", "bv_device.h", "bv_scan.h", "bv_slots.h", "bv_mfma.h", "bv_exact.h", "bv_sort.h",
-           "bv_host.h", "bv_embed.h", "bv_embed_device.h", "bv_finish.h", "bv_rows_device.h",
+           "bv_host.h", "bv_embed.h", "bv_embed_device.h", "bv_finish.h", "bv_linear_q8_plan.h", "bv_rows_device.h",
            "bv_attention_device.h"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

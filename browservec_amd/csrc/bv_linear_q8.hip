@@ -8,6 +8,7 @@
 #include "bv_embed.h"
 #include "bv_embed_device.h"
 #include "bv_finish.h"
+#include "bv_linear_q8_plan.h"
 #include "bv_mfma.h"
 
 #include <algorithm>
@@ -459,45 +460,23 @@ hipError_t rows_of(const LinearQ8Args &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Shapes of tiles, and when one is done with m rows: `fix` and rounds of the tiles that
-// the card holds at a time, each a + b k and what its activations take; the last round
-// of fewer tiles is `part` hundredths of one and their share of the rest (ns, fitted to
-// 40..32768 x 384..4096 x 384..4096 without an activation, within 3 to 7%: the shapes
-// chosen take 1.3% more than each size's best).  32768 x 1024, k 1024: 50.5 us in the last,
-// the others 53.4, 59.2, 60.8, 75.4, 113, 107 and 141; 2037 x 768, k 768: 17.6, 12.6, 14.7,
-// 11.8, 8.8, 7.5, 7.6 and 10.7; 200 x 1024, k 4096: 51, 39, 43, 35, 26, 18, 14 and 11.
-struct Shape {
-    uint32_t bm, bn, cus, part, fix, a, b, gelu;  // cus: tiles of a compute unit
-};
-constexpr int SHAPES = 8;
-constexpr Shape shapes[SHAPES] = {{64, 64, 1, 80, 2150, 2906, 163, 470},    {64, 64, 2, 55, 2391, 2494, 375, 750},
-                                  {64, 128, 1, 80, 2116, 3082, 361, 940},   {128, 128, 1, 85, 1883, 2968, 585, 1880},
-                                  {128, 256, 1, 80, 1815, 5220, 845, 3760}, {192, 256, 1, 75, 1829, 7617, 1105, 4400},
-                                  {128, 256, 2, 45, 2504, 7446, 1590, 3000}, {256, 256, 1, 70, 2947, 7700, 1389, 7500}};
-uint64_t done_in(const LinearQ8Args &a, uint64_t m, const Shape &t) {
-    const uint64_t tiles = ((m + t.bm - 1) / t.bm) * ((a.n + t.bn - 1) / t.bn), at_a_time = 256 * t.cus, rest = tiles % at_a_time;
-    const uint64_t rounds = tiles / at_a_time * 100 + (rest ? t.part + (100 - t.part) * rest / at_a_time : 0);
-    return t.fix + rounds * (t.a + (uint64_t)t.b * a.k / 100 + (a.act > 1 ? t.gelu : 0)) / 100;
-}
-uint64_t done_in(const LinearQ8Args &a, uint64_t m, int *shape) {
-    uint64_t least = ~0ull;
-    for (int i = 0; i < SHAPES; i++) {
-        const uint64_t ns = done_in(a, m, shapes[i]);
-        if (ns < least) least = ns, *shape = i;
-    }
-    return least;
+// Shape I's tiles: its rows, columns and step from the plan's table, waves across, buffers, groups.
+template <class O, int I, int WN, int ST, int KG = 1>
+hipError_t shape(const LinearQ8Args &a, hipStream_t s) {
+    constexpr Q8Shape t = q8_shapes[I];
+    return tile_of<O, t.bm, t.bn, WN, t.bk, ST, KG>(a, s);
 }
 template <class O>
-hipError_t shape_of(const LinearQ8Args &a, int shape, hipStream_t s) {
-    switch (shape) {
-    case 0: return tile_of<O, 64, 64, 2, 512, 2, 4>(a, s);
-    case 1: return tile_of<O, 64, 64, 2, 256, 2, 2>(a, s);
-    case 2: return tile_of<O, 64, 128, 2, 256, 2, 2>(a, s);
-    case 3: return tile_of<O, 128, 128, 4, 128, 4>(a, s);
-    case 4: return tile_of<O, 128, 256, 4, 128, 3>(a, s);
-    case 5: return tile_of<O, 192, 256, 4, 128, 2>(a, s);
-    case 6: return tile_of<O, 128, 256, 4, 64, 3>(a, s);
-    default: return tile_of<O, 256, 256, 4, 128, 2>(a, s);
+hipError_t shape_of(const LinearQ8Args &a, int i, hipStream_t s) {
+    switch (i) {
+    case 0: return shape<O, 0, 2, 2, 4>(a, s);
+    case 1: return shape<O, 1, 2, 2, 2>(a, s);
+    case 2: return shape<O, 2, 2, 2, 2>(a, s);
+    case 3: return shape<O, 3, 4, 4>(a, s);
+    case 4: return shape<O, 4, 4, 3>(a, s);
+    case 5: return shape<O, 5, 4, 2>(a, s);
+    case 6: return shape<O, 6, 4, 3>(a, s);
+    default: return shape<O, 7, 4, 2>(a, s);
     }
 }
 
@@ -534,22 +513,9 @@ hipError_t linear_q8_of(LinearQ8Args a, void *ws, hipStream_t s) {
     // Results that pass the L2s' 32 MB twice over go by them, and leave them to x and w:
     // 32768 x 4096, k 1024, bf16 192 -> 176 us, with GELU 251 -> 226.
     a.once = a.m * a.n * sizeof(O) > (64u << 20);
-    // Whole rounds of tiles in one shape, and the rows that are left in another, where
-    // that is done first.  20011 x 1024, k 4096: 16384 rows in 256 x 256 tiles and 3627 in 128 x
-    // 128, 135 -> 125 us; 16492 x 1024, k 1024, GELU: 42.3 -> 37.9.  2 us: what the second launch adds.
-    int shape = 0, then = 0;
-    uint64_t rows = a.m, least = done_in(a, a.m, &shape);
-    for (int i = 0; i < SHAPES; i++) {
-        const Shape &t = shapes[i];
-        const uint64_t tiles_n = (a.n + t.bn - 1) / t.bn, at_a_time = 256 * t.cus;
-        const uint64_t whole = (a.m + t.bm - 1) / t.bm * tiles_n / at_a_time * at_a_time / tiles_n * t.bm;
-        if (whole == 0 || whole >= a.m) continue;
-        int j;
-        const uint64_t ns = done_in(a, whole, t) + done_in(a, a.m - whole, &j) + 2000;
-        if (ns < least) least = ns, rows = whole, shape = i, then = j;
-    }
-    const hipError_t e = shape_of<O>(part_of<O>(a, 0, rows, 0, a.n), shape, s);
-    return e != hipSuccess || rows == a.m ? e : shape_of<O>(part_of<O>(a, rows, a.m - rows, 0, a.n), then, s);
+    const Q8Plan p = q8_plan(a.m, a.n, a.k, a.act);
+    const hipError_t e = shape_of<O>(part_of<O>(a, 0, p.rows, 0, a.n), p.shape, s);
+    return e != hipSuccess || p.rows == a.m ? e : shape_of<O>(part_of<O>(a, p.rows, a.m - p.rows, 0, a.n), p.then, s);
 }
 
 }  // namespace
