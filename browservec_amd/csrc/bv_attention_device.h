@@ -388,15 +388,16 @@ __device__ __forceinline__ void store_by_rows(const AttentionArgs &a, const Plac
 // waiting.  At D = 64 (96 x 1..512 tokens, 12 heads over 4: 46 us causal, 58
 // without a mask) they are busy for 12 and 38%: what is left is the chain at a
 // workgroup's start, offsets, queries and first keys one after the other.
-//   Registers spilled by a lane: with turns 3 at D = 128 and 23 at D = 256 (with a
-// window 3 and 22, outside the loop's common path).  4 x 4096 tokens, 8 heads, no
-// mask: d = 128 344 us, at odd addresses 791; d = 104 330, d = 100, whose elements are
-// loaded one by one, 1453; d = 256 1229, at odd addresses 2714.
+//   Registers spilled by a lane: with turns 3 or 4 at D = 128 and 23 at D = 256, with a
+// window or without, outside the loop's common path.  4 x 4096 tokens, 8 heads, no mask:
+// d = 128 339 us, with heads one element apart from odd addresses on 888; d = 104 329, d =
+// 100, whose elements are loaded one by one, 1475; d = 256 1295, one element apart 2830.
 //   A window: 32768 tokens, 8 heads of 128 over 2, the last 4096 keys and 4 first ones, f16,
-// 565 to 591 us by card, 870 to 910 TFLOP/s of visible pairs; 6% more are computed, in tiles
-// that the window cuts and the first keys' own.  4 x 4001..8192 tokens, 16 heads over 4, the last
-// 512 keys: d = 64 90 to 103 us, of which half does not grow with the window (1024 keys
-// 150); d = 32 70, with four workgroups a CU (one register spilled), 77 with three.
+// 564 us a call (593 under the profiler), 910 TFLOP/s of visible pairs; 6% more are computed,
+// in tiles that the window cuts and the first keys' own; one element apart 1053.  4 x
+// 4001..8192 tokens, 16 heads over 4, the last 512 keys: d = 64 88 to 97 us by card, of which
+// half does not grow with the window (1024 keys 143 to 155); d = 32 64 to 68, with four
+// workgroups a CU (two registers spilled; three took 10% longer).
 template <class T, int D, int KT, int GROUPS, bool DIRECT, bool LOCAL>
 __global__ __launch_bounds__(256 * GROUPS, LOCAL && D <= 32 ? 4 : D <= 128 ? 2 : 1) void attention_tile(AttentionArgs a, AttentionPlan pl,
                                                                                  uint64_t first) {

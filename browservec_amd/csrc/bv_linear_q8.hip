@@ -36,15 +36,15 @@ __device__ __forceinline__ float bias_at(const LinearQ8Args &a, uint32_t n) {
 // multiplies those of the 32 before, and waits for the next tile before it
 // multiplies a tile's last 32, already in registers.
 //
-// Bound by the card's power and the end of a tile.  8192 x 8192 x 8192: 460 to 480 us,
-// 2.3 POP/s (the library's bare product 453): the matrix cores are busy for 60% of the cycles
-// at 1.8 GHz; without loads 385, without LDS reads as well 324.  32768 x 4096, k 1024,
-// bf16: the loop takes 127 us, all of it 168 (the library's bare product 195), with
-// bias and GELU 200, of which the activation's 13 instructions a result are 30 to 50.  20011 x
-// 1024, k 4096, onto a residual of 32 bits 122: 1.6 rounds of tiles.  Tried and slower:
-// groups of waves that take turns between LDS and matrix cores (482), four waves of 128 x 128 (539),
-// 192 x 128 tiles two a CU (535); steps of 64 codes ask the L2 for half lines and are
-// bound by its requests (580), but two such workgroups a CU cover each other's ends.
+// Bound by the card's power and the end of a tile.  8192 x 8192 x 8192: 470 to 490 us by
+// card, 2.3 POP/s (the library's bare product 450): the matrix cores are busy for 60% of the
+// cycles at 1.8 GHz; without loads 385, without LDS reads as well 324.  32768 x 4096, k 1024,
+// bf16: the loop takes 127 us, all of it 166 (the library's bare product 194), with
+// bias and GELU 195 to 215, of which the activation's 13 instructions a result are 30 to 50.
+// 20011 x 1024, k 4096, onto a residual of 32 bits: 114 to 126 in two launches.  Tried and
+// slower: groups of waves that take turns between LDS and matrix cores (482), four waves of
+// 128 x 128 (539), 192 x 128 tiles two a CU (535); steps of 64 codes ask the L2 for half lines
+// and are bound by its requests (580), but two such workgroups a CU cover each other's ends.
 //
 // LDS rows hold BK codes, in 16-byte chunks; chunk c of row r lies at
 // c ^ swizzle(r), so that sixteen lanes that read the same chunk of consecutive
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(128 * WN * KG, BM * BN / WN > 16384 ? 1 : 2) void l
 // Up to 16 * MF rows of x (one question, a few): w is read once, straight into
 // the matrix instructions' registers, 16 of its rows a workgroup; the waves
 // split k and join their sums in LDS.  Bound by latency: a wave waits for four
-// steps' loads before it starts the next four (9 x 1536, k 384: 2.8 us; 8 x 4096, k 4096, 5.6:
-// 16.8 MB of w at 3.0 TB/s).
+// steps' loads before it starts the next four (9 x 1536, k 384: 3.7 us; 8 x 4096, k 4096, 6.3:
+// 16.8 MB of w at 2.7 TB/s).
 constexpr uint32_t ROW_WAVES = 8;
 template <class O, int MF>
 __global__ __launch_bounds__(ROW_WAVES * 64) void linear_q8_rows(LinearQ8Args a) {
@@ -375,7 +375,9 @@ __global__ __launch_bounds__(ROW_WAVES * 64) void linear_q8_rows(LinearQ8Args a)
 
 // ---------------------------------------------------------------- packing --
 // Rows for linear_q8_tile, which loads 16 bytes at 16-byte addresses: k rounded
-// up to 16 with zeros.  x's and w's in one launch (114 x 1000, k 820: 9.9 us, in two 12.1).
+// up to 16 with zeros, by every call: nothing is kept.  x's and w's in one launch (114 x
+// 1000, k 820: 8.5 us, 2 more in two).  20011 x 1024, k 4090, onto a residual of 32 bits: 150
+// us, k 4096 114; of w alone 120; 32768 x 4096, k 1000, GELU: 224, k 1008 209.
 struct PackJob {
     const int8_t *from;
     int8_t *to;
@@ -405,8 +407,8 @@ __global__ __launch_bounds__(256) void pack_codes(PackJob a, PackJob b, uint32_t
     }
 }
 
-// Rows up to which w goes straight to the registers: 32 rows of 4096 x 4096 8.1 us,
-// 33 by tiles 8.7; of 768 x 768 3.4 and 5.3.
+// Rows up to which w goes straight to the registers: 32 rows of 4096 x 4096 8.3 us,
+// 33 by tiles 10.8; of 768 x 768 3.4 and 4.3.
 constexpr uint64_t FEW_ROWS = 32;
 // A tile's loads have 32-bit offsets: 256 rows of as many codes reach 2^31
 // bytes.  Rows further apart are packed; k itself is far below.

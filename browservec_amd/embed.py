@@ -188,7 +188,9 @@ class EmbedOps:
         [..., k] with a float32 scale a row (``norm_q8`` gives both), weight int8 [n,
         k] with a scale a row ([n]; ``norm_q8`` with kind None), bias [n] of any float
         type, residual and the result [..., n] of one float type: out_dtype, or out's
-        or residual's, or bfloat16.  k at most 131071."""
+        or residual's, or bfloat16.  k at most 131071.  More than 32 rows of x: where k
+        is no multiple of 16, or rows do not begin at multiples of 16 bytes, every call
+        copies them, so keep weights padded with zeros to such a k, and x with them."""
         a, address = self._linear_q8
         act = ACTIVATIONS.get(activation)
         if act is None:

@@ -404,7 +404,9 @@ int bv_embed_linear(bv_embed *e, const bv_embed_linear_args *args);
  * or BV_BF16), residual and y [m][n] in out_dtype (of the three as well).  bias and
  * residual may be NULL; residual may be y itself.  k is at most 131071: up to there
  * the sums are exact in 32 bits; they are rounded to a 32-bit float and multiplied
- * by x's scale, then by w's. */
+ * by x's scale, then by w's.  With more than 32 rows of x, matrices whose k is no
+ * multiple of 16, or whose address or stride is none, are laid out anew by every
+ * call, weights too: keep those padded with zeros to a k that is one. */
 typedef struct bv_embed_linear_q8_args {
     uint32_t size;        /* sizeof(bv_embed_linear_q8_args) */
     uint32_t out_dtype;
@@ -600,7 +602,8 @@ int bv_embed_norm(bv_embed *e, const bv_embed_norm_args *args);
  * norm is of t in 32 bits.  residual may be NULL (total is then, too): t = x.
  * y [tokens][dim] in out_dtype; with BV_I8 the row's codes
  *   q = round(y 127 / top), ties to even, with the scale top / 127 in scales
- *   [tokens] (32-bit floats), top the row's largest |y|:
+ *   [tokens] (32-bit floats), top the row's largest |y| (computed as y times 127 /
+ *   top, each rounded to 32 bits: next to a half q may be either neighbour):
  * what bv_embed_linear_q8 takes (weights too, with BV_NORM_NONE).  A row of zeros
  * has scale 0; one that holds an infinity or NaN codes 0 and a scale of NaN.  total
  * may be residual, or x where it has its type, and y may be x, each with the same
